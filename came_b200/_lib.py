@@ -12,7 +12,7 @@ _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "libcame_b200.so")
 
 DT_F32, DT_F16, DT_BF16 = 0, 1, 2
-MODE_FP32, MODE_TILE8, MODE_FLAT8 = 0, 1, 2
+MODE_FP32, MODE_TILE8, MODE_FLAT8, MODE_ADAMW, MODE_ADAMW8 = 0, 1, 2, 3, 4
 
 F_SQ_FIX = 1 << 0
 F_SQ_CLAMP = 1 << 1
@@ -23,6 +23,7 @@ F_WD_MUL2 = 1 << 5
 F_WD_ADD2 = 1 << 6
 F_UPDATE_F16 = 1 << 7
 F_RSQRT_CLAMP = 1 << 8
+F_ADAMW_CLIP = 1 << 9
 
 MAX_GROUPS = 64
 KERNEL_COUNT = 20
@@ -55,7 +56,11 @@ class CameHyper(C.Structure):
     ]
 
 
-assert C.sizeof(CameTensorDesc) == 136 and C.sizeof(CameHyper) == 64
+class CameGradRef(C.Structure):
+    _fields_ = [("g", C.c_void_p), ("n", C.c_int64), ("dtype", C.c_int32), ("reserved", C.c_int32)]
+
+
+assert C.sizeof(CameTensorDesc) == 136 and C.sizeof(CameHyper) == 64 and C.sizeof(CameGradRef) == 24
 
 # name -> (restype, argtypes); every symbol include/came_b200.h declares
 SYMBOLS = {
@@ -72,6 +77,10 @@ SYMBOLS = {
     "came_b200_plan_set_pointers": (C.c_int, [C.c_void_p, C.POINTER(C.c_void_p), C.POINTER(C.c_void_p), C.c_int,
                                                C.c_void_p]),
     "came_b200_step": (C.c_int, [C.c_void_p, C.POINTER(CameHyper), C.c_int, C.c_void_p]),
+    "came_b200_plan_norm_offset": (C.c_int64, [C.c_void_p]),
+    "came_b200_clip_workspace_bytes": (C.c_size_t, [C.c_int]),
+    "came_b200_clip_grad_norm": (C.c_int, [C.POINTER(CameGradRef), C.c_int, C.c_float, C.c_void_p, C.c_void_p, C.c_size_t,
+                                           C.c_void_p]),
     "came_b200_plan_set_hyper": (C.c_int, [C.c_void_p, C.POINTER(CameHyper), C.c_int]),
     "came_b200_peer_copy_async": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_int, C.c_void_p]),
     "came_b200_ipc_export": (C.c_int, [C.c_void_p, C.c_char_p, C.POINTER(C.c_uint64)]),

@@ -60,7 +60,9 @@ struct LaunchItem {
 };
 
 inline int elem_bytes(int dt) { return dt == CAME_DT_F32 ? 4 : 2; }
-inline bool is_nd(const CameTensorDesc& d) { return d.cols != 0 && d.batch > 1; }
+inline bool is_adamw(const CameTensorDesc& d) { return d.mode == CAME_MODE_ADAMW || d.mode == CAME_MODE_ADAMW8; }
+inline bool is_nd(const CameTensorDesc& d) { return d.cols != 0 && d.batch > 1 && !is_adamw(d); }
+inline int64_t elements(const CameTensorDesc& d) { return d.rows * (d.cols ? d.cols : 1) * (d.batch > 1 ? (int64_t)d.batch : 1); }
 inline int nd_chunk(const CameTensorDesc& d) { return is_nd(d) && !disable_fast() ? nd_small_batch(d.rows, d.cols) : 0; }
 
 // Which kernels take the passes of a matrix.
@@ -73,6 +75,12 @@ struct VecFlags {
 
 VecFlags vec_flags(const CameTensorDesc& d, bool fast) {
     VecFlags f{0, 0, 0};
+    if (is_adamw(d)) {      // eight elements of every tensor by one access of their own size each
+        auto on = [](const void* p, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; };
+        const uintptr_t state = d.mode == CAME_MODE_ADAMW ? 32 : 8;
+        f.v = on(d.p, 8 * elem_bytes(d.p_dtype)) && on(d.g, 8 * elem_bytes(d.g_dtype)) && on(d.m, state) && on(d.sq_row, state) ? 8 : 1;
+        return f;
+    }
     if (d.cols == 0 || is_nd(d)) return f;      // 1-D and N-D tensors have kernels of their own
     const bool aligned = aligned16(d.g) && aligned16(d.m) && aligned16(d.p);
     f.v = aligned && d.cols % 8 == 0 ? 8 : 1;
@@ -104,7 +112,8 @@ constexpr long long SMALL_SET_ELEMS = 16 << 20;
 struct Context {
     bool small;      // the whole-step kernel takes every matrix
     int bands;       // its bands of 16 rows per warp
-    bool generic(const CameTensorDesc& d) const { return d.cols != 0 && !is_nd(d) && (small || !vec_flags(d).wide); }
+    int chunk;       // elements of an AdamW item
+    bool generic(const CameTensorDesc& d) const { return d.cols != 0 && !is_nd(d) && !is_adamw(d) && (small || !vec_flags(d).wide); }
 };
 
 int64_t generic_tiles(const CameTensorDesc& d, int bands) {
@@ -114,6 +123,17 @@ int64_t generic_tiles(const CameTensorDesc& d, int bands) {
 size_t partial_floats(int64_t n) { return (size_t)(n + cdiv(n, PARTIAL_GROUP) + 1); }
 size_t partial_counters(int64_t n) { return (size_t)(1 + cdiv(n, PARTIAL_GROUP)); }
 
+// AdamW: 2048 elements (8 for each thread of a CTA) per item in small sets, so that all SMs have some; more where there are
+// items enough, so that a CTA sets up for more work.
+int adamw_chunk(const CameTensorDesc* descs, int n) {
+    double total = 0.0;
+    for (int i = 0; i < n; ++i)
+        if (is_adamw(descs[i])) total += (double)elements(descs[i]);
+    int chunk = 2048;
+    while (chunk < 16384 && total / chunk > 16.0 * 148) chunk *= 2;
+    return chunk;
+}
+
 Context context(const CameTensorDesc* descs, int n) {
     const char* e = getenv("CAME_B200_SMALL_SET_ELEMS");
     const double line = e ? atof(e) : (double)SMALL_SET_ELEMS;
@@ -121,7 +141,7 @@ Context context(const CameTensorDesc* descs, int n) {
     for (int i = 0; i < n; ++i)
         if (vec_flags(descs[i]).wide)
             staged += (double)descs[i].rows * (double)descs[i].cols * (descs[i].mode == CAME_MODE_FLAT8 ? 4.0 / 3.0 : 1.0);
-    Context c{staged < line, 16};
+    Context c{staged < line, 16, adamw_chunk(descs, n)};
     auto items = [&](int bands) {
         int64_t tiles = 0;
         for (int i = 0; i < n; ++i)
@@ -154,6 +174,10 @@ Geometry geometry(const CameTensorDesc& d, const Context& ctx) {
     Geometry g{};
     g.R = d.rows;
     g.C = d.cols;
+    if (is_adamw(d)) {      // flat_chunks: items
+        g.flat_chunks = cdiv(elements(d), ctx.chunk);
+        return g;
+    }
     g.nbR = (int)cdiv(g.R, QBLOCK);
     if (d.cols == 0) return g;
     if (is_nd(d)) {      // nbR / nbC: blocks of the flattened row / column vectors; flat_chunks: flat blocks of 256 elements
@@ -187,7 +211,9 @@ size_t carve(const CameTensorDesc& d, const Geometry& g, const Context& ctx, flo
     };
     Scratch s{};
     s.nbR = g.nbR;
-    if (d.cols == 0) {
+    if (is_adamw(d)) {
+        s.g_v = vec_flags(d).v;
+    } else if (d.cols == 0) {
         s.spart = take((size_t)g.nbR);      // block partials of sum u^2
         s.scal = take(4);
         s.counters = reinterpret_cast<int32_t*>(take(4));
@@ -257,10 +283,16 @@ int validate(const CameTensorDesc& d, int i) {
     if (!d.p || !d.g || !d.m) return fail(CAME_E_INVALID, "tensor %d: p, g and m must be non-null", i);
     if (d.rows <= 0 || d.cols < 0) return fail(CAME_E_INVALID, "tensor %d: bad shape [%lld, %lld]", i, (long long)d.rows, (long long)d.cols);
     if (d.rows > 0x7fffffffLL || d.cols > 0x7fffffffLL) return fail(CAME_E_UNSUPPORTED, "tensor %d: dimension above 2^31-1", i);
-    if (d.mode < CAME_MODE_FP32 || d.mode > CAME_MODE_FLAT8) return fail(CAME_E_INVALID, "tensor %d: bad mode %d", i, d.mode);
+    if (d.mode < CAME_MODE_FP32 || d.mode > CAME_MODE_ADAMW8) return fail(CAME_E_INVALID, "tensor %d: bad mode %d", i, d.mode);
     if (d.p_dtype < CAME_DT_F32 || d.p_dtype > CAME_DT_BF16 || d.g_dtype < CAME_DT_F32 || d.g_dtype > CAME_DT_BF16)
         return fail(CAME_E_INVALID, "tensor %d: bad dtype", i);
     if (d.group < 0 || d.group >= MAX_GROUPS) return fail(CAME_E_INVALID, "tensor %d: group %d outside [0, %d)", i, d.group, MAX_GROUPS);
+    if (is_adamw(d)) {
+        if (!d.sq_row || !d.res_row) return fail(CAME_E_INVALID, "tensor %d: AdamW needs exp_avg_sq (sq_row) and a step count (res_row)", i);
+        if (d.mode == CAME_MODE_ADAMW8 && (!d.m_absmax || !d.sq_row_absmax)) return fail(CAME_E_INVALID, "tensor %d: missing scales", i);
+        const double n = (double)d.rows * (double)(d.cols ? d.cols : 1) * (double)(d.batch > 1 ? d.batch : 1);
+        return n > 4.0e12 ? fail(CAME_E_UNSUPPORTED, "tensor %d: too many elements", i) : CAME_OK;      // (items are counted in 32 bits)
+    }
     const bool quant = d.mode != CAME_MODE_FP32;
     if (quant && !d.m_absmax) return fail(CAME_E_INVALID, "tensor %d: 8-bit exp_avg needs m_absmax", i);
     if (!d.sq_row || (quant && !d.sq_row_absmax)) return fail(CAME_E_INVALID, "tensor %d: missing exp_avg_sq state", i);
@@ -280,7 +312,7 @@ int validate(const CameTensorDesc& d, int i) {
 }
 
 struct Layout {
-    size_t off_descs, off_scr, off_hyp, off_status, off_bar, off_sync, off_work, off_float, total;
+    size_t off_descs, off_scr, off_hyp, off_status, off_bar, off_sync, off_norm, off_work, off_float, total;
     size_t n_work;
 };
 
@@ -288,6 +320,10 @@ size_t count_work(const CameTensorDesc* descs, int n, const Context& ctx) {
     size_t w = 0;
     for (int i = 0; i < n; ++i) {
         const Geometry g = geometry(descs[i], ctx);
+        if (is_adamw(descs[i])) {      // its items, and one entry for its step count
+            w += (size_t)g.flat_chunks + 1;
+            continue;
+        }
         if (descs[i].cols == 0) {
             w += (size_t)g.nbR;
             continue;
@@ -308,7 +344,8 @@ size_t count_work(const CameTensorDesc* descs, int n, const Context& ctx) {
     return w;
 }
 
-constexpr int MAX_GENERIC_LAUNCHES = 32;      // (gradient type, parameter type, layout) combinations: 27
+constexpr int MAX_GENERIC_LAUNCHES = 64;      // (gradient type, parameter type, layout) combinations: 27, and 18 of AdamW
+constexpr int NORM_LINE = 256;                // bytes in front of the partial sums: the norm itself
 
 Layout layout(const CameTensorDesc* descs, int n, const Context& ctx) {
     Layout L{};
@@ -319,6 +356,15 @@ Layout layout(const CameTensorDesc* descs, int n, const Context& ctx) {
     L.off_status = off; off = align_up(off + sizeof(int));
     L.off_sync = off;  off = align_up(off + (2 * (size_t)n + 12) * sizeof(int));   // fused kernel: per-tensor item counters, list cursors
     L.off_bar = off;   off = align_up(off + MAX_GENERIC_LAUNCHES * sizeof(uint32_t));      // grid barriers of the whole-step kernel
+    bool clip = false;
+    int64_t adamw_items = 0;
+    for (int i = 0; i < n; ++i)
+        if (is_adamw(descs[i])) {
+            clip = clip || (descs[i].flags & CAME_F_ADAMW_CLIP);
+            adamw_items += geometry(descs[i], ctx).flat_chunks;
+        }
+    L.off_norm = off;
+    if (clip) off = align_up(off + NORM_LINE + (size_t)grad_norm_parts((int)std::min<int64_t>(adamw_items, 1 << 30)) * sizeof(double));
     L.n_work = count_work(descs, n, ctx);
     L.off_work = off;  off = align_up(off + L.n_work * sizeof(Work));
     L.off_float = off;
@@ -364,6 +410,9 @@ struct came_plan {
     std::vector<char> pushable;    // ... or by the whole-step kernel, which serves the push mode too
     std::vector<char> push_must;   // pushable whatever the size of the set: has to lie in the local buffer (else it is not pushed)
     bool needs_hyp = false;        // some kernel reads the hyper-parameters from the workspace
+    int adamw_chunk = 0;
+    bool adamw_clip = false;
+    int norm_parts = 0;            // partial sums of the gradient norm
     int n_push = 0;                // push mode: peers that receive every parameter the fused kernel updates
     long long push_delta[MAX_PUSH_PEERS] = {};
     uintptr_t push_lo = 0, push_hi = 0;      // the local buffer the pushed parameters must lie in
@@ -451,6 +500,13 @@ int came_b200_plan_create(const CameTensorDesc* descs, int n_tensors, void* work
         const int rc = validate(descs[i], i);
         if (rc != CAME_OK) return rc;
     }
+    int n_adamw = 0, n_clip = 0;
+    for (int i = 0; i < n_tensors; ++i)
+        if (is_adamw(descs[i])) {
+            ++n_adamw;
+            n_clip += descs[i].flags & CAME_F_ADAMW_CLIP ? 1 : 0;
+        }
+    if (n_clip != 0 && n_clip != n_adamw) return fail(CAME_E_INVALID, "plan_create: CAME_F_ADAMW_CLIP on %d of %d AdamW tensors", n_clip, n_adamw);
     const Context ctx = context(descs, n_tensors);
     const Layout L = layout(descs, n_tensors, ctx);
     if (!workspace || (reinterpret_cast<uintptr_t>(workspace) % ALIGN) != 0)
@@ -498,9 +554,9 @@ int came_b200_plan_create(const CameTensorDesc* descs, int n_tensors, void* work
         }
     };
     const CameTensorDesc* D = descs;
-    auto is1d = [&](int i) { return D[i].cols == 0; };
+    auto is1d = [&](int i) { return D[i].cols == 0 && !is_adamw(D[i]); };
     auto isgen = [&](int i) { return ctx.generic(D[i]); };
-    auto is2d = [&](int i) { return D[i].cols != 0 && !is_nd(D[i]) && !isgen(i); };      // staged
+    auto is2d = [&](int i) { return D[i].cols != 0 && !is_adamw(D[i]) && !is_nd(D[i]) && !isgen(i); };      // staged
     auto isnd = [&](int i) { return is_nd(D[i]); };
     auto nokey = [&](int) { return Key{0, 0, 0, 0}; };
     const auto& vf = plan->vflags;
@@ -544,6 +600,39 @@ int came_b200_plan_create(const CameTensorDesc* descs, int n_tensors, void* work
             std::tie(it.work3_off, it.n3) = list(mats, [&](int i) { return geo[i].flat_chunks; });
             std::tie(it.work4_off, it.n4) = list(kv.second.second, [&](int i) { return (int64_t)geo[i].nbR; });
             plan->launches.push_back(it);
+        }
+    }
+    // AdamW: one launch per (gradient type, parameter type, layout); their items lie one behind the other
+    {
+        std::map<Key, std::vector<int>> groups;
+        for (int i = 0; i < n_tensors; ++i)
+            if (is_adamw(D[i])) groups[Key{D[i].g_dtype, D[i].p_dtype, D[i].mode, 0}].push_back(i);
+        plan->adamw_chunk = ctx.chunk;
+        plan->adamw_clip = n_clip > 0;
+        const size_t first_item = work.size();
+        if (plan->adamw_clip) plan->launches.push_back(LaunchItem{KID_GRAD_NORM, {}, first_item, 0, 0, 0, 0, 0, 0, 0, 0});
+        const size_t first_launch = plan->launches.size();
+        for (auto& kv : groups) {
+            LaunchItem it{};
+            it.kernel = std::get<2>(kv.first) == CAME_MODE_ADAMW8 ? KID_ADAMW8 : KID_ADAMW;
+            it.key = KernelKey{std::get<0>(kv.first), std::get<1>(kv.first), std::get<2>(kv.first), 0};
+            it.bar = (int)plan->launches.size();
+            it.work_off = work.size();
+            for (int i : kv.second)
+                for (int64_t t = 0; t < geo[i].flat_chunks; ++t) work.push_back(Work{i, (int32_t)t});
+            it.n = (int)(work.size() - it.work_off);
+            plan->launches.push_back(it);
+        }
+        if (plan->adamw_clip) {      // the norm takes the items of all of them
+            plan->launches[first_launch - 1].n = (int)(work.size() - first_item);
+            plan->norm_parts = grad_norm_parts((int)(work.size() - first_item));
+        }
+        size_t k = first_launch;
+        for (auto& kv : groups) {
+            LaunchItem& it = plan->launches[k++];
+            it.work2_off = work.size();
+            it.n2 = (int)kv.second.size();
+            for (int i : kv.second) work.push_back(Work{i, 0});
         }
     }
     // tensors of more than two dimensions
@@ -700,7 +789,8 @@ int came_b200_plan_create(const CameTensorDesc* descs, int n_tensors, void* work
         delete plan;
         return fail(CAME_E_CUDA, "plan_create: %s", cudaGetErrorString(e));
     }
-    for (const LaunchItem& it : plan->launches) plan->needs_hyp = plan->needs_hyp || it.kernel != KID_GENERIC;
+    for (const LaunchItem& it : plan->launches)
+        plan->needs_hyp = plan->needs_hyp || (it.kernel != KID_GENERIC && it.kernel != KID_ADAMW && it.kernel != KID_ADAMW8 && it.kernel != KID_GRAD_NORM);
     *out = plan;
     return CAME_OK;
 }
@@ -809,6 +899,7 @@ int came_b200_step(came_plan_t* plan, const CameHyper* hypers, int n_groups, cam
     // The whole-step kernel takes a few records as kernel arguments; a captured step reads them from memory, so that a
     // replay sees new values.
     const bool by_value = !capturing && n_groups <= GENERIC_MAX_HYP;
+    static_assert(GENERIC_MAX_HYP == ADAMW_MAX_HYP, "one rule for the records that travel as arguments");
     cudaError_t e = cudaSuccess;
     if (plan->needs_hyp || !by_value) {
         e = cudaMemcpyAsync(plan->ws + plan->L.off_hyp, src, (size_t)n_groups * sizeof(CameHyper), cudaMemcpyHostToDevice, st);
@@ -827,6 +918,7 @@ int came_b200_step(came_plan_t* plan, const CameHyper* hypers, int n_groups, cam
         if (e != cudaSuccess) return fail(CAME_E_CUDA, "step: counter reset: %s", cudaGetErrorString(e));
     }
     int launches = 0, fused_launches = 0;
+    double* const norm_parts = reinterpret_cast<double*>(plan->ws + plan->L.off_norm + NORM_LINE);
     for (const LaunchItem& it : plan->launches) {
         came_plan::Timed tm{it.kernel, nullptr, nullptr};
         if (timing) {
@@ -834,7 +926,15 @@ int came_b200_step(came_plan_t* plan, const CameHyper* hypers, int n_groups, cam
                 return fail(CAME_E_CUDA, "step: cudaEventCreate failed");
             cudaEventRecord(tm.t0, st);
         }
-        if (it.kernel == KID_GENERIC) {
+        if (it.kernel == KID_GRAD_NORM)
+            e = launch_grad_norm(a, wbase + it.work_off, it.n, plan->adamw_chunk, by_value ? norm : nullptr, n_groups, norm_parts, st);
+        else if (it.kernel == KID_ADAMW || it.kernel == KID_ADAMW8) {
+            const AdamwArgs w{wbase + it.work_off, wbase + it.work2_off, it.n, it.n2, plan->adamw_chunk, 0,
+                              reinterpret_cast<uint32_t*>(plan->ws + plan->L.off_bar) + it.bar, plan->adamw_clip ? norm_parts : nullptr,
+                              reinterpret_cast<float*>(plan->ws + plan->L.off_norm), plan->norm_parts};
+            e = launch_adamw(it.key, a, w, by_value ? norm : nullptr, n_groups, st);
+        }
+        else if (it.kernel == KID_GENERIC) {
             const GenericLists l{wbase + it.work_off, wbase + it.work2_off, wbase + it.work3_off, wbase + it.work4_off,
                                  it.n, it.n2, it.n3, it.n4, reinterpret_cast<uint32_t*>(plan->ws + plan->L.off_bar) + it.bar};
             e = launch_generic(it.key, a, by_value ? norm : nullptr, n_groups, l, st);
@@ -857,6 +957,25 @@ int came_b200_step(came_plan_t* plan, const CameHyper* hypers, int n_groups, cam
     }
     plan->last_launches = launches;
     return CAME_OK;
+}
+
+int64_t came_b200_plan_norm_offset(const came_plan_t* plan) { return plan && plan->adamw_clip ? (int64_t)plan->L.off_norm : -1; }
+
+size_t came_b200_clip_workspace_bytes(int n_tensors) { return n_tensors < 0 ? 0 : clip_parts(n_tensors) * sizeof(double); }
+
+int came_b200_clip_grad_norm(const CameGradRef* grads, int n_tensors, float max_norm, float* norm, void* workspace,
+                             size_t workspace_bytes, came_stream_t stream) {
+    if (n_tensors < 0 || (n_tensors > 0 && !grads) || !norm) return fail(CAME_E_INVALID, "clip_grad_norm: null argument or negative count");
+    if (!(max_norm >= 0.0f)) return fail(CAME_E_INVALID, "clip_grad_norm: max_norm must be >= 0");
+    for (int i = 0; i < n_tensors; ++i) {
+        if (grads[i].n < 0 || (grads[i].n > 0 && !grads[i].g)) return fail(CAME_E_INVALID, "clip_grad_norm: tensor %d: null pointer or negative size", i);
+        if (grads[i].dtype < CAME_DT_F32 || grads[i].dtype > CAME_DT_BF16) return fail(CAME_E_INVALID, "clip_grad_norm: tensor %d: bad dtype", i);
+        if (grads[i].n > 4000000000000LL) return fail(CAME_E_UNSUPPORTED, "clip_grad_norm: tensor %d: too many elements", i);
+    }
+    if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 8 != 0 || workspace_bytes < came_b200_clip_workspace_bytes(n_tensors))
+        return fail(CAME_E_WORKSPACE, "clip_grad_norm: workspace of %zu bytes, 8-byte aligned, needed", came_b200_clip_workspace_bytes(n_tensors));
+    const cudaError_t e = launch_clip(grads, n_tensors, max_norm, norm, static_cast<double*>(workspace), (cudaStream_t)stream);
+    return e == cudaSuccess ? CAME_OK : fail(CAME_E_CUDA, "clip_grad_norm: %s", cudaGetErrorString(e));
 }
 
 int came_b200_peer_copy_async(void* dst, const void* src, size_t bytes, int src_device, came_stream_t stream) {
@@ -964,7 +1083,7 @@ int came_b200_plan_read_timing(came_plan_t* plan, float* ms, int* launches) {
 const char* came_b200_kernel_name(int kernel) {
     static const char* names[CAME_KERNEL_COUNT] = {
         "sq_partials", "sq_finalize", "sumsq", "s_finalize", "moment", "res_finalize",
-        "apply", "generic", "apply_flat", "?", "?", "?", "nd_sq", "nd_mean", "nd_sumsq", "nd_s", "nd_res",
+        "apply", "generic", "apply_flat", "adamw", "adamw8", "grad_norm", "nd_sq", "nd_mean", "nd_sumsq", "nd_s", "nd_res",
         "nd_resmean", "nd_apply", "moment_apply"};
     return (kernel >= 0 && kernel < CAME_KERNEL_COUNT) ? names[kernel] : "?";
 }

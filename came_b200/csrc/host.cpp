@@ -3,7 +3,8 @@
 // A step of a few hundred small tensors is over on the GPU before Python has looked at every parameter's gradient:
 // walking 528 parameters (two data_ptr() calls, a dtype and a shape each) takes 280 us in Python, 15 us here.  What is
 // here: the check that the tensor table of the previous step still stands, the new gradient addresses when only those
-// moved, the hyper-parameter records, the step call itself; and the codec functions' allocation and launch.  Everything
+// moved, the hyper-parameter records, the step call itself; the codec functions' allocation and launch; and the walk over the
+// gradients, allocation and launches of clip_grad_norm_.  Everything
 // else (first step, changed tensors, states, errors) stays in optim.py / engine.py, to which `step` hands over by
 // returning SLOW.
 #define PY_SSIZE_T_CLEAN
@@ -15,6 +16,8 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
+#include <cmath>
 #include <memory>
 #include <string>
 #include <vector>
@@ -53,6 +56,8 @@ struct StepTable {
     std::vector<std::vector<Param>>* groups;
     std::vector<Plan>* plans;
     std::vector<PyObject*>* states;      // state dicts that carry a "step" count (owned)
+    bool adamw;                          // records of AdamW: one per group
+    double max_norm;
     PyObject *k_params, *k_lr, *k_betas, *k_eps, *k_clip, *k_wd, *k_scale, *k_step, *one;
 };
 
@@ -91,7 +96,7 @@ bool usable(const at::Tensor& p, const at::Tensor& g) {
     return g.layout() == at::kStrided && g.is_contiguous() && p.is_contiguous() && g.numel() == p.numel();
 }
 
-// build(param_groups, [(DevicePlan, device index, n)], [state dict]): remembers the tensors of a step that the
+// build(param_groups, [(DevicePlan, device index, n)], [state dict][, max_grad_norm of AdamW]): remembers the tensors of a step that the
 // Python path has just made.  Parameters with a gradient fill the plans' tables in order, by device.  False when they do not.
 bool build(StepTable* s, PyObject* groups, PyObject* plans, PyObject* states) {
     table_clear(s);
@@ -149,7 +154,10 @@ PyObject* table_build(PyObject* self, PyObject* args) {
     HANDLE_TH_ERRORS
     StepTable* s = reinterpret_cast<StepTable*>(self);
     PyObject *groups, *plans, *states;
-    if (!PyArg_ParseTuple(args, "O!O!O!", &PyList_Type, &groups, &PyList_Type, &plans, &PyList_Type, &states)) return nullptr;
+    double max_norm = -1.0;
+    if (!PyArg_ParseTuple(args, "O!O!O!|d", &PyList_Type, &groups, &PyList_Type, &plans, &PyList_Type, &states, &max_norm)) return nullptr;
+    s->adamw = max_norm > 0.0;
+    s->max_norm = max_norm;
     bool ok = false;
     try {
         ok = build(s, groups, plans, states);
@@ -208,6 +216,35 @@ bool hypers_of(StepTable* s, PyObject* group, CameHyper* out) {
     return true;
 }
 
+// The record of an AdamW group (engine.make_adamw_hyper)
+bool adamw_hyper_of(StepTable* s, PyObject* group, CameHyper* h) {
+    double lr, betas[2], eps, wd, scale = 1.0;
+    if (!number(group, s->k_lr, &lr) || !numbers(group, s->k_betas, betas, 2) || !number(group, s->k_eps, &eps) ||
+        !number(group, s->k_wd, &wd))
+        return false;
+    if (PyDict_GetItemWithError(group, s->k_scale) && !number(group, s->k_scale, &scale)) return false;
+    *h = CameHyper{};
+    float* beta[2] = {&h->beta1, &h->beta2};
+    float* om[2] = {&h->om_beta1, &h->om_beta2};
+    float* ln[2] = {&h->beta3, &h->om_beta3};
+    for (int k = 0; k < 2; ++k) {
+        if (!(betas[k] >= 0.0 && betas[k] < 1.0)) return false;
+        *beta[k] = (float)betas[k];
+        *om[k] = (float)(1.0 - betas[k]);
+        const double l = std::log(betas[k]);      // (-inf at zero)
+        *ln[k] = (float)l;
+        h->reserved[k] = betas[k] > 0.0 ? (float)(l - (double)*ln[k]) : 0.0f;
+    }
+    h->lr = (float)lr;
+    h->eps0 = (float)eps;
+    h->weight_decay = (float)wd;
+    h->wd_lr = (float)(wd * lr);
+    h->decay_mul = (float)(1.0 - lr * wd);
+    h->clip_threshold = (float)s->max_norm;
+    h->grad_scale = (float)scale;
+    return true;
+}
+
 // The plan as it stands, null when it has been closed (PyErr set on an error)
 came_plan_t* handle_of(const Plan& plan) {
     PyObject* h = PyObject_GetAttrString(plan.py, "handle");      // ctypes.c_void_p or None
@@ -223,7 +260,8 @@ came_plan_t* handle_of(const Plan& plan) {
 long step(StepTable* s, PyObject* groups) {
     if (s->plans->empty() || !PyList_Check(groups) || (size_t)PyList_GET_SIZE(groups) != s->groups->size()) return SLOW;
     const size_t n_groups = s->groups->size();
-    if (2 * n_groups > 64) return SLOW;
+    const size_t records = (s->adamw ? 1 : 2) * n_groups;
+    if (records > 64) return SLOW;
     // (what is used without the lock below: the table may be dropped or rebuilt by another thread meanwhile)
     struct Target {
         came_plan_t* handle;
@@ -268,7 +306,8 @@ long step(StepTable* s, PyObject* groups) {
     }
     CameHyper hyp[64];
     for (size_t gi = 0; gi < n_groups; ++gi)
-        if (!hypers_of(s, PyList_GET_ITEM(groups, (Py_ssize_t)gi), hyp + 2 * gi)) {
+        if (!(s->adamw ? adamw_hyper_of(s, PyList_GET_ITEM(groups, (Py_ssize_t)gi), hyp + gi)
+                       : hypers_of(s, PyList_GET_ITEM(groups, (Py_ssize_t)gi), hyp + 2 * gi))) {
             PyErr_Clear();      // the Python path raises what there is to raise
             return SLOW;
         }
@@ -295,7 +334,7 @@ long step(StepTable* s, PyObject* groups) {
     NoGil unlocked;
     for (const Target& t : targets) {
         c10::cuda::CUDAGuard guard(t.device);
-        const int rc = came_b200_step(t.handle, hyp, (int)(2 * n_groups), c10::cuda::getCurrentCUDAStream(t.device).stream());
+        const int rc = came_b200_step(t.handle, hyp, (int)records, c10::cuda::getCurrentCUDAStream(t.device).stream());
         if (rc != CAME_OK) return FAILED + rc;
         launches += came_b200_plan_last_launches(t.handle);
     }
@@ -383,8 +422,52 @@ PyObject* dequantize(PyObject*, PyObject* args) {
     END_HANDLE_TH_ERRORS
 }
 
+// clip_grad_norm([tensor], max_norm, of parameters): the norm, or None where the caller has to look closer (a gradient that
+// is no dense CUDA tensor of a type the kernels take, another device, the same gradient twice, no gradient at all)
+PyObject* clip_grad_norm(PyObject*, PyObject* args) {
+    HANDLE_TH_ERRORS
+    PyObject* list;
+    double max_norm;
+    int of_params;
+    if (!PyArg_ParseTuple(args, "O!dp", &PyList_Type, &list, &max_norm, &of_params)) return nullptr;
+    std::vector<CameGradRef> refs;
+    at::Tensor first;
+    std::vector<at::Tensor> keep;      // (another thread may drop a gradient while the lock is released)
+    for (Py_ssize_t i = 0; i < PyList_GET_SIZE(list); ++i) {
+        const at::Tensor& t = tensor_of(PyList_GET_ITEM(list, i));
+        const at::Tensor& g = of_params ? t.grad() : t;
+        if (!g.defined()) continue;
+        if (g.layout() != at::kStrided || !g.is_cuda() || (first.defined() && g.device() != first.device())) Py_RETURN_NONE;
+        const at::ScalarType type = g.scalar_type();
+        const int dtype = type == at::kFloat ? CAME_DT_F32 : type == at::kHalf ? CAME_DT_F16 : type == at::kBFloat16 ? CAME_DT_BF16 : -1;
+        if (dtype < 0 || !g.is_non_overlapping_and_dense()) Py_RETURN_NONE;
+        if (!first.defined()) first = g;
+        if (g.numel() > 0) refs.push_back(CameGradRef{const_cast<void*>(g.const_data_ptr()), g.numel(), dtype, 0});
+        keep.push_back(g);
+    }
+    if (!first.defined()) Py_RETURN_NONE;
+    std::vector<const void*> sorted;
+    for (const CameGradRef& r : refs) sorted.push_back(r.g);
+    std::sort(sorted.begin(), sorted.end());
+    if (std::adjacent_find(sorted.begin(), sorted.end()) != sorted.end()) Py_RETURN_NONE;
+    at::Tensor norm;
+    int rc;
+    {
+        NoGil unlocked;
+        c10::cuda::CUDAGuard guard(first.device());
+        const size_t bytes = came_b200_clip_workspace_bytes((int)refs.size());
+        norm = at::empty({}, first.options().dtype(at::kFloat).requires_grad(false));
+        const at::Tensor ws = at::empty({(int64_t)bytes}, norm.options().dtype(at::kByte));
+        rc = came_b200_clip_grad_norm(refs.data(), (int)refs.size(), (float)max_norm, norm.mutable_data_ptr<float>(), ws.mutable_data_ptr(),
+                                      bytes, stream_of(norm));
+    }
+    return status(rc, rc == CAME_OK ? THPVariable_Wrap(norm) : nullptr);
+    END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef module_methods[] = {{"quantize", quantize, METH_VARARGS, "(tensor, signed, tile) -> (codes, absmax)"},
                                 {"dequantize", dequantize, METH_VARARGS, "(codes, absmax, signed, tile) -> fp32"},
+                                {"clip_grad_norm", clip_grad_norm, METH_VARARGS, "([tensor], max_norm, of parameters) -> norm or None"},
                                 {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_host", "native host side of came_b200", -1, module_methods, nullptr, nullptr, nullptr, nullptr};
 

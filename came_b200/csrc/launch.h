@@ -42,7 +42,10 @@ enum KernelId {
     KID_APPLY,
     KID_GENERIC,           // whole step of small sets, odd shapes and 1-D tensors (generic.cu)
     KID_APPLY_FLAT,
-    KID_ND_SQ = 12,        // tensors of more than two dimensions (nd.cu); 9 to 11 are free, the numbers are part of the C interface
+    KID_ADAMW,             // AdamW (adamw.cu): states in fp32, in float8, sums of squares of all gradients (gradnorm.cu)
+    KID_ADAMW8,
+    KID_GRAD_NORM,
+    KID_ND_SQ,             // tensors of more than two dimensions (nd.cu); the numbers are part of the C interface
     KID_ND_MEAN,
     KID_ND_SUMSQ,
     KID_ND_S,
@@ -96,6 +99,29 @@ int nd_small_kb(int64_t rows, int64_t cols);
 // the same for 3 x 3 and 1 x 1 (nd_fixed.cu); key: element types, mode = 8-bit states | 3 x 3 << 1
 int nd_fixed_batch(int64_t rows, int64_t cols);
 cudaError_t launch_nd_fixed(int kernel, const KernelKey& key, const StepArgs& a, const Work* work, int n, cudaStream_t st);
+// AdamW (adamw.cu): one launch per (gradient type, parameter type, layout)
+struct AdamwArgs {
+    const Work* work;           // chunks of the tensors
+    const Work* tensors;        // the tensors themselves, whose step counts the last CTA raises
+    int n, n_tensors;
+    int chunk;                  // elements of an item (a multiple of 2048)
+    int by_value;
+    uint32_t* ticket;           // CTAs that are through (zero between launches)
+    const double* norm_parts;   // partial sums of the squared gradients, or null: no clip
+    float* norm_out;
+    int n_parts;
+};
+constexpr int ADAMW_MAX_HYP = 8;      // hyper-parameter records that travel as kernel arguments
+cudaError_t launch_adamw(const KernelKey& key, const StepArgs& a, const AdamwArgs& w, const CameHyper* host_hyp, int n_hyp,
+                         cudaStream_t st);
+// gradient norm (gradnorm.cu).  Sums of squares of the plan's AdamW gradients: parts[0 .. grad_norm_parts(n))
+int grad_norm_parts(int n);
+cudaError_t launch_grad_norm(const StepArgs& a, const Work* work, int n, int chunk, const CameHyper* host_hyp, int n_hyp, double* parts,
+                             cudaStream_t st);
+// the same for tensors given by value, then (unless max_norm is infinite) their scaling in place
+size_t clip_parts(int n_tensors);      // doubles of workspace
+cudaError_t launch_clip(const CameGradRef* grads, int n, float max_norm, float* norm, double* parts, cudaStream_t st);
+
 cudaError_t launch_selftest_grid_barrier(int* words, cudaStream_t st);
 cudaError_t launch_selftest_bounded_wait(int* status, int* observed, cudaStream_t st);
 

@@ -48,8 +48,11 @@ class Entry:
 
     def structure_key(self):
         """Everything except the p / g addresses: a change here needs a new plan."""
-        return (tuple(self.p.shape), self.p.dtype, self.g.dtype, self.mode, self.flags, self.group,
-                self.m.data_ptr(), self.sq_row.data_ptr())
+        key = (tuple(self.p.shape), self.p.dtype, self.g.dtype, self.mode, self.flags, self.group,
+               self.m.data_ptr(), self.sq_row.data_ptr())
+        if self.mode in (_lib.MODE_ADAMW, _lib.MODE_ADAMW8):
+            key += (self.res_row.data_ptr(), _ptr(self.m_absmax), _ptr(self.sq_row_absmax))
+        return key
 
 
 def _ptr(t):
@@ -83,6 +86,34 @@ def make_hyper(lr, betas, eps, clip_threshold, weight_decay, *, python_scalars: 
     return h
 
 
+def make_adamw_hyper(lr, betas, eps, weight_decay, max_grad_norm=None, grad_scale: float = 1.0) -> CameHyper:
+    """The record of an AdamW param_group: scalars formed in double and rounded once; ln beta as the sum of two fp32 numbers,
+    from which the device forms 1 - beta^t in double."""
+    f = np.float32
+    h = CameHyper()
+    b = [float(x) for x in betas]
+    if len(b) != 2 or not all(0.0 <= x < 1.0 for x in b):
+        raise ValueError(f"betas must be two numbers in [0, 1), got betas={betas}")
+    h.lr = f(lr)
+    h.beta1, h.beta2 = f(b[0]), f(b[1])
+    h.om_beta1, h.om_beta2 = f(1.0 - b[0]), f(1.0 - b[1])
+    for k, x in enumerate(b):
+        ln = math.log(x) if x > 0.0 else -math.inf
+        hi = f(ln)
+        h.reserved[k] = f(ln - float(hi)) if x > 0.0 else f(0.0)
+        if k == 0:
+            h.beta3 = hi
+        else:
+            h.om_beta3 = hi
+    h.eps0 = f(eps)
+    h.weight_decay = f(weight_decay)
+    h.wd_lr = f(float(weight_decay) * float(lr))
+    h.decay_mul = f(1.0 - float(lr) * float(weight_decay))
+    h.clip_threshold = f(1.0 if max_grad_norm is None else max_grad_norm)
+    h.grad_scale = f(grad_scale)
+    return h
+
+
 class DevicePlan:
     """A came_plan_t and the workspace it lives in, for the tensors of one device."""
 
@@ -92,9 +123,13 @@ class DevicePlan:
         self.n = len(entries)
         self.structure = tuple(e.structure_key() for e in entries)
         self.addresses = tuple((e.p.data_ptr(), e.g.data_ptr()) for e in entries)
+        # AdamW: the plan keeps the states it points at
+        self.keep = [(e.m, e.m_absmax, e.sq_row, e.sq_row_absmax, e.res_row) for e in entries
+                     if e.mode in (_lib.MODE_ADAMW, _lib.MODE_ADAMW8)]
         descs = (CameTensorDesc * self.n)()
         for d, e in zip(descs, entries):
-            if e.p.dim() < 1:
+            elementwise = e.mode in (_lib.MODE_ADAMW, _lib.MODE_ADAMW8)
+            if e.p.dim() < 1 and not elementwise:
                 raise NotImplementedError("came_b200 does not step 0-dimensional tensors")
             d.p, d.g = e.p.data_ptr(), e.g.data_ptr()
             d.m, d.m_absmax = _ptr(e.m), _ptr(e.m_absmax)
@@ -102,8 +137,8 @@ class DevicePlan:
             d.sq_col, d.sq_col_absmax = _ptr(e.sq_col), _ptr(e.sq_col_absmax)
             d.res_row, d.res_row_absmax = _ptr(e.res_row), _ptr(e.res_row_absmax)
             d.res_col, d.res_col_absmax = _ptr(e.res_col), _ptr(e.res_col_absmax)
-            if e.p.dim() == 1:
-                d.rows, d.cols, d.batch = e.p.shape[0], 0, 0
+            if e.p.dim() <= 1:
+                d.rows, d.cols, d.batch = e.p.numel(), 0, 0
             else:      # more than two dimensions: a batch of [shape[-2], shape[-1]] matrices
                 d.rows, d.cols = e.p.shape[-2], e.p.shape[-1]
                 d.batch = math.prod(e.p.shape[:-2]) if e.p.dim() > 2 else 0
@@ -159,6 +194,12 @@ class DevicePlan:
         """Rewrites the hyper-parameter records a captured step uploads at every replay (no stream work)."""
         arr = (CameHyper * len(hypers))(*hypers)
         _lib.check(self.lib.came_b200_plan_set_hyper(self.handle, arr, len(hypers)))
+
+    @property
+    def grad_norm(self):
+        """The norm the last step clipped by, as a view of the workspace (None: the plan takes none)."""
+        at = self.lib.came_b200_plan_norm_offset(self.handle)
+        return None if at < 0 else self.workspace[at:at + 4].view(torch.float32).reshape(())
 
     @property
     def last_launches(self) -> int:

@@ -13,6 +13,9 @@ class would have taken on a CUDA device:
     CAME8bitFull     flat layout, came_kernels.cu:4792-5248  flat layout, came_kernels.cu:4172-4255
     CAME8bitMemory   flat layout                             flat layout, fp16 update (4257-4340)
 
+    AdamW            element-wise, fp32 states (no counterpart in the reference, as the next one)
+    AdamW8bit        element-wise, float8 states with a power-of-two scale per 256 elements
+
 All tensors of a step are handed to the library in one call; there is no per-tensor launch loop, no
 scratch tensor in the optimizer state and no CPU / eager fallback: parameters must live on a CUDA device.
 """
@@ -27,7 +30,7 @@ import torch
 import torch.optim
 
 from . import _host, _lib
-from .engine import Entry, StepEngine, make_hyper
+from .engine import Entry, StepEngine, make_adamw_hyper, make_hyper
 
 BLOCK = 256
 TILE = 16
@@ -168,6 +171,9 @@ class _CameB200Optimizer(torch.optim.Optimizer):
     with layout in {"fp", "tile", "flat"} and variant 0 (kernel-style fp32 scalars) or 1 (Python-style)."""
 
     _fp_mode_tag = None
+    _family = "CAME"
+    _records = 2              # hyper-parameter records per param_group
+    _elementwise = False      # AdamW: any shape, step counts in device memory
 
     def __init__(self, params, defaults):
         super().__init__(params, defaults)
@@ -217,7 +223,14 @@ class _CameB200Optimizer(torch.optim.Optimizer):
             keep.append(g_data)
         e = Entry(p=p_data, g=g_data, mode=0, flags=flags, group=group_index, keep=keep)
         factored = p.dim() >= 2
-        if layout == "fp":
+        if layout == "adamw":
+            e.mode = _lib.MODE_ADAMW
+            e.m, e.sq_row, e.res_row = state["exp_avg"], state["exp_avg_sq"], state["step"]
+        elif layout == "adamw8":
+            e.mode = _lib.MODE_ADAMW8
+            e.m, e.m_absmax = state["exp_avg_q"], state["exp_avg_scale"]
+            e.sq_row, e.sq_row_absmax, e.res_row = state["exp_avg_sq_q"], state["exp_avg_sq_scale"], state["step"]
+        elif layout == "fp":
             e.mode = _lib.MODE_FP32
             e.m = state["exp_avg"]
             if factored:
@@ -241,26 +254,28 @@ class _CameB200Optimizer(torch.optim.Optimizer):
     def _collect(self):
         entries, hypers, copy_backs = [], self._hypers(), []
         for gi, group in enumerate(self.param_groups):
-            if gi >= _lib.MAX_GROUPS // 2:
-                raise RuntimeError(f"came_b200 supports at most {_lib.MAX_GROUPS // 2} param_groups")
+            if gi >= _lib.MAX_GROUPS // self._records:
+                raise RuntimeError(f"came_b200 supports at most {_lib.MAX_GROUPS // self._records} param_groups")
             for p in group["params"]:
                 if p.grad is None:
                     continue
                 if p.grad.is_sparse:
-                    raise RuntimeError("CAME does not support sparse gradients.")
+                    raise RuntimeError(f"{self._family} does not support sparse gradients.")
                 grad = p.grad
                 if not p.is_cuda:
                     raise RuntimeError(
                         "came_b200 steps CUDA tensors only (there is no CPU fallback); "
                         f"got a parameter on {p.device}")
-                if p.dim() == 0:
+                if self._elementwise and p.numel() == 0:
+                    continue
+                if p.dim() == 0 and not self._elementwise:
                     raise NotImplementedError("came_b200 does not step 0-dimensional parameters")
                 layout, flags, variant = self._route(p, grad, group)
                 state = self.state[p]
                 self._prepare_state(p, state, layout)
-                if "step" in state:
+                if "step" in state and not self._elementwise:
                     state["step"] += 1
-                e, cb = self._entry(p, grad, state, layout, flags, 2 * gi + variant)
+                e, cb = self._entry(p, grad, state, layout, flags, self._records * gi + variant)
                 entries.append(e)
                 if cb is not None:
                     copy_backs.append(cb)
@@ -286,12 +301,16 @@ class _CameB200Optimizer(torch.optim.Optimizer):
         self._table = None
         if not entries or copy_backs or any(e.keep for e in entries):
             return
-        stepped = [self.state[p] for g in self.param_groups for p in g["params"]
-                   if p.grad is not None and "step" in self.state[p]]
+        stepped = [] if self._elementwise else [self.state[p] for g in self.param_groups for p in g["params"]
+                                                if p.grad is not None and "step" in self.state[p]]
         plans = [(plan, plan.device.index, plan.n) for plan in self._engine.plans.values()]
         table = _host.StepTable()
-        if all(isinstance(g["params"], list) for g in self.param_groups) and table.build(self.param_groups, plans, stepped):
+        if all(isinstance(g["params"], list) for g in self.param_groups) and \
+                table.build(self.param_groups, plans, stepped, *self._table_args()):
             self._table = table
+
+    def _table_args(self) -> tuple:
+        return ()
 
     def _step_again(self) -> bool:
         """Steps the remembered table; False when the full path has to be taken."""
@@ -354,7 +373,7 @@ class _CameB200Optimizer(torch.optim.Optimizer):
         for group in self.param_groups:
             for p in group["params"]:
                 st = self.state.get(p)
-                if st is not None and "step" in st and p.grad is not None:
+                if st is not None and "step" in st and p.grad is not None and not self._elementwise:
                     st["step"] -= 1   # _collect counted a step that did not run
         if entries:
             self._engine.prepare(entries)
@@ -624,3 +643,147 @@ class CAME8bit2D(_CameB200Optimizer):
 
     def _route(self, p, grad, group):
         return "tile", _FLAGS_TILE8, 0
+
+
+# ----------------------------------------------------------------------------------------------
+# AdamW
+# ----------------------------------------------------------------------------------------------
+
+class AdamW(_CameB200Optimizer):
+    """AdamW with decoupled weight decay, states in fp32 whatever the parameters' type (float32, float16, bfloat16):
+
+        m = b1 m + (1 - b1) c g,  v = b2 v + (1 - b2) (c g)^2,  c = grad_scale * min(1, max_grad_norm / (N + 1e-6))
+        p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+
+    State keys are those of `torch.optim.AdamW` (`step`, `exp_avg`, `exp_avg_sq`; its checkpoints load, without amsgrad and
+    maximize); `step` is a tensor on the parameter's device, raised by the kernel, so that a captured step counts its
+    replays.  A param_group may carry `grad_scale` (default 1), by which every gradient is multiplied as it is read.
+
+    max_grad_norm: clip by the norm N of all gradients of the optimizer (each times its group's grad_scale), as the step
+    reads them: the gradients themselves are not written.  N is left in `grad_norm`.  With a norm that is not finite nothing
+    is stepped and no count raised.  `math.inf` takes the norm without clipping.  All parameters have to be on one device.
+
+    Parameters of any shape (empty ones are passed over).  States replaced by hand (not by load_state_dict) are seen after
+    the next `prime_for_cuda_graph()`."""
+
+    _family = "AdamW"
+    _records = 1
+    _elementwise = True
+    _layout = "adamw"
+
+    def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, *,
+                 max_grad_norm=None):
+        if isinstance(lr, torch.Tensor):
+            raise ValueError("lr must be a number, got a tensor")
+        if not lr >= 0.0:
+            raise ValueError(f"lr must be >= 0, got {lr}")
+        if len(betas) != 2 or not all(0.0 <= b < 1.0 for b in betas):
+            raise ValueError(f"betas must be two numbers in [0, 1), got betas={betas}")
+        if not eps >= 0.0:
+            raise ValueError(f"eps must be >= 0, got {eps}")
+        if not weight_decay >= 0.0:
+            raise ValueError(f"weight_decay must be >= 0, got {weight_decay}")
+        self._max_grad_norm = None
+        defaults = dict(lr=float(lr), betas=(float(betas[0]), float(betas[1])), eps=float(eps), weight_decay=float(weight_decay))
+        super().__init__(params, defaults)
+        self.max_grad_norm = max_grad_norm
+
+    @property
+    def max_grad_norm(self):
+        return self._max_grad_norm
+
+    @max_grad_norm.setter
+    def max_grad_norm(self, value) -> None:
+        if value is not None and not float(value) > 0.0:
+            raise ValueError(f"max_grad_norm must be > 0 or None, got {value}")
+        self._max_grad_norm = None if value is None else float(value)
+        self._table = None
+
+    @property
+    def grad_norm(self):
+        """Norm of all gradients at the last step under `max_grad_norm`: a 0-dimensional fp32 tensor on the device, which the
+        next step overwrites (clone it to keep it).  None without `max_grad_norm`, and before the first step."""
+        plans = list(self._engine.plans.values())
+        return plans[0].grad_norm if self._max_grad_norm is not None and len(plans) == 1 else None
+
+    def _route(self, p, grad, group):
+        return self._layout, _lib.F_ADAMW_CLIP if self._max_grad_norm is not None else 0, 0
+
+    def _hypers(self):
+        return [make_adamw_hyper(g["lr"], g["betas"], g["eps"], g["weight_decay"], self._max_grad_norm,
+                                 float(g.get("grad_scale", 1.0))) for g in self.param_groups]
+
+    def _table_args(self) -> tuple:
+        return (1.0 if self._max_grad_norm is None else self._max_grad_norm,)
+
+    _state_tensors = {"exp_avg": torch.float32, "exp_avg_sq": torch.float32}
+
+    def _init_state(self, state, p) -> None:
+        for key, dtype in self._state_tensors.items():
+            state[key] = torch.zeros(tuple(p.shape), device=p.device, dtype=dtype)
+
+    def _prepare_state(self, p, state, layout) -> None:
+        if len(state) == 0:
+            state["step"] = torch.zeros((), device=p.device, dtype=torch.float32)
+            self._init_state(state, p)
+        for key in ("step", *self._state_tensors):
+            if key not in state:
+                raise RuntimeError(f"the state of a parameter has no {key!r}: it is another optimizer's")
+        for key, dtype in self._state_tensors.items():
+            t = state[key]
+            if tuple(t.shape) != tuple(p.shape):
+                raise RuntimeError(f"Parameter shape changed: {key} is {tuple(t.shape)}, the parameter {tuple(p.shape)}")
+            if t.dtype != dtype or t.device != p.device or not t.is_contiguous():
+                raise RuntimeError(f"{key} has to be a contiguous {dtype} tensor on {p.device}, got {t.dtype} on {t.device}")
+        t = state["step"]
+        if not torch.is_tensor(t) or t.numel() != 1 or t.dtype != torch.float32 or t.device != p.device:
+            raise RuntimeError(f"step has to be an fp32 tensor of one element on {p.device}")
+
+    def _collect(self):
+        entries, hypers, copy_backs = super()._collect()
+        if self._max_grad_norm is not None and len({e.p.device for e in entries}) > 1:
+            raise RuntimeError("max_grad_norm needs all parameters on one device")
+        return entries, hypers, copy_backs
+
+    def load_state_dict(self, state_dict):
+        for g in state_dict["param_groups"]:
+            for key in ("amsgrad", "maximize"):
+                if g.get(key, False):
+                    raise ValueError(f"came_b200.{type(self).__name__} has no {key}")
+        super().load_state_dict(state_dict)
+        for group in self.param_groups:
+            for p in group["params"]:
+                st = self.state.get(p)
+                if not st:
+                    continue
+                if "step" in st:
+                    st["step"] = torch.as_tensor(st["step"], dtype=torch.float32, device=p.device).reshape(()).clone()
+                if self._layout == "adamw":      # torch keeps them in the parameter's type
+                    for key in ("exp_avg", "exp_avg_sq"):
+                        if torch.is_tensor(st.get(key)):
+                            st[key] = st[key].to(dtype=torch.float32, memory_format=torch.contiguous_format).contiguous()
+
+
+class AdamW8bit(AdamW):
+    """AdamW with two bytes of state per element.  Per block of 256 flat elements the first moment is held as float8 e4m3
+    codes (`exp_avg_q`), the second as e5m2 codes (`exp_avg_sq_q`), each with a power-of-two scale in one e8m0 byte
+    (`exp_avg_scale`, `exp_avg_sq_scale`): the value is `code.float() * scale.float()`.  Both are rounded stochastically, with
+    bits hashed from the element's index and the step count: two runs give the same bits.  Rounded to nearest, the second
+    moment could not follow at betas[1] = 0.999, where a step moves it by less than half a spacing.  The update itself uses
+    the moments before they are rounded."""
+
+    _layout = "adamw8"
+    _state_tensors = {"exp_avg_q": torch.float8_e4m3fn, "exp_avg_sq_q": torch.float8_e5m2}
+    _scales = ("exp_avg_scale", "exp_avg_sq_scale")
+
+    def _init_state(self, state, p) -> None:
+        super()._init_state(state, p)
+        for key in self._scales:
+            state[key] = torch.ones((_num_blocks(p.numel()),), device=p.device, dtype=torch.float32).to(torch.float8_e8m0fnu)
+
+    def _prepare_state(self, p, state, layout) -> None:
+        super()._prepare_state(p, state, layout)
+        for key in self._scales:
+            t = state.get(key)
+            if t is None or t.numel() < _num_blocks(p.numel()) or t.dtype != torch.float8_e8m0fnu or t.device != p.device or not t.is_contiguous():
+                raise RuntimeError(f"{key} has to hold {_num_blocks(p.numel())} float8_e8m0fnu scales on {p.device}")

@@ -276,6 +276,7 @@ class ShardedStepper:
         for b in range(sharded.n_buckets):
             ps = [params_by_index[i] for i in sharded.owned_in_bucket(b)]
             self.opts.append(make_optimizer(ps) if ps else None)
+        self._check_clip()
         self.peer = None
         self.gather_mode = "nccl"
         if gather_mode != "nccl" and sharded.world_size > 1:
@@ -347,7 +348,13 @@ class ShardedStepper:
                 lst.append((lo, view.numel()))
         self._push_ranges = ranges
 
+    def _check_clip(self) -> None:
+        if (self.sharded.world_size > 1 or self.sharded.n_buckets > 1) and \
+                any(getattr(o, "max_grad_norm", None) is not None for o in self.opts):
+            raise ValueError("max_grad_norm is the norm of one optimizer's gradients; here each holds a part of them")
+
     def step(self, gather: bool = True):
+        self._check_clip()
         works = []
         if self.gather_mode == "push":
             if self._push_ranges is None:
@@ -464,6 +471,7 @@ class Zero1Step:
 
     def run(self) -> None:
         s = self.sharded
+        self.stepper._check_clip()
         if self.stepper.gather_mode == "push":
             self._run_push()
             return

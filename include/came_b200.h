@@ -37,8 +37,13 @@ enum {
     CAME_MODE_FP32 = 0,  /* CAMECUDA: fp32 exp_avg and fp32 row/col vectors (CAMECUDA.py:83-100)              */
     CAME_MODE_TILE8 = 1, /* CAME8bit / CAME8bit2D 2-D: int8 exp_avg, one absmax per 16x16 tile, uint8 vectors  */
                          /* with one absmax per 256 (came8bit2d_state.py:33-55)                                */
-    CAME_MODE_FLAT8 = 2  /* CAME8bitFull / CAME8bitMemory, and every 1-D 8-bit tensor: int8 exp_avg with one   */
+    CAME_MODE_FLAT8 = 2, /* CAME8bitFull / CAME8bitMemory, and every 1-D 8-bit tensor: int8 exp_avg with one   */
                          /* absmax per 256 flat elements, uint8 vectors (blockwise_quantization.py:17-27)      */
+    /* AdamW (no counterpart in the reference).  Element-wise: rows, cols and batch only give the element count. */
+    CAME_MODE_ADAMW = 3, /* fp32 exp_avg (m) and exp_avg_sq (sq_row)                                           */
+    CAME_MODE_ADAMW8 = 4 /* exp_avg: float8 e4m3 codes (m), exp_avg_sq: float8 e5m2 codes (sq_row), each with  */
+                         /* one e8m0 byte (a power-of-two scale) per 256 flat elements in m_absmax / sq_row_absmax */
+                         /* (pointers to bytes there); rounded stochastically, see came_b200_step              */
 };
 
 /* per-tensor arithmetic variants; each reproduces one of the reference's code paths */
@@ -52,6 +57,8 @@ enum {
                                        /* neither: one rounding            (came_kernels.cu:2505-2510)          */
 #define CAME_F_UPDATE_F16    (1u << 7) /* 1-D: u rounded to fp16 before use (came_kernels.cu:1069-1122)         */
 #define CAME_F_RSQRT_CLAMP   (1u << 8) /* 1-D: rsqrt(max(v,1e-30))         (came_kernels.cu:1041, CAMECUDA.py:267)*/
+#define CAME_F_ADAMW_CLIP    (1u << 9) /* AdamW: clip by the norm of all AdamW gradients of the plan (all of them carry */
+                                       /* the flag, or none); a norm that is not finite leaves the step out          */
 
 /*
  * One tensor of the optimizer.  cols == 0 marks a 1-D (non-factored) tensor of `rows` elements, whose
@@ -68,7 +75,7 @@ typedef struct CameTensorDesc {
     float* sq_row_absmax; /* [ceil(rows/256)]                                     */
     void* sq_col;         /* exp_avg_sq_col [cols]                                */
     float* sq_col_absmax;
-    void* res_row;        /* exp_avg_res_row [rows]                               */
+    void* res_row;        /* exp_avg_res_row [rows]; AdamW: fp32 step count [1], raised by the step */
     float* res_row_absmax;
     void* res_col;        /* exp_avg_res_col [cols]                               */
     float* res_col_absmax;
@@ -105,6 +112,12 @@ typedef struct CameHyper {
                                         /* scale, say: saves the trainer's separate unscale pass over g); 0 means 1   */
     float reserved[2];
 } CameHyper;
+/*
+ * AdamW tensors read a record as follows: lr, beta1, beta2, om_beta1, om_beta2, wd_lr and grad_scale as above; eps0 = eps
+ * (added to the root of the second moment); clip_threshold = largest norm of all gradients (CAME_F_ADAMW_CLIP; may be
+ * infinite); beta3 / om_beta3 = ln beta1 / ln beta2 rounded to fp32, reserved[0] / reserved[1] = what that rounding left of
+ * them (the bias corrections 1 - beta^t are formed in 64 bits from the step count in device memory).
+ */
 
 typedef struct came_plan came_plan_t;
 
@@ -155,6 +168,39 @@ int came_b200_plan_set_pointers(came_plan_t* plan, const void* const* g, void* c
  * param_update (1406, 1589, 1507, 1675), came_full_nonfactored_step[_fp16_update] (856, 916).
  */
 int came_b200_step(came_plan_t* plan, const CameHyper* hypers, int n_groups, came_stream_t stream);
+/*
+ * AdamW tensors, with c = grad_scale (times min(1, clip_threshold / (N + 1e-6)) under CAME_F_ADAMW_CLIP, N the norm of all
+ * gradients, each times its group's grad_scale) and t the step count after this step:
+ *     m' = beta1 m + (1 - beta1) c g          v' = beta2 v + (1 - beta2) (c g)^2
+ *     p' = p (1 - lr wd) - lr / (1 - beta1^t) * m' / (sqrt(v') / sqrt(1 - beta2^t) + eps)
+ * p' uses m' and v' before they are rounded to float8.  CAME_MODE_ADAMW8 holds a block of 256 flat elements as code * 2^k:
+ * 2^k puts the exponent of the largest magnitude at 2^7 (m) resp. 2^14 (v), at least k = -126; y = x / 2^k, for v no less
+ * than 2^-16 unless the whole block is zero, is rounded to the format after a number r has been added to its fp32 bits and
+ * the low 20 (m) / 21 (v) bits have been cleared: with h = mix((e >> 3) + mix(t)) * (0x9E3779B1 * (2 (e & 7) + 1)) mod 2^32,
+ * e the flat index of the element and mix the 32-bit mixer x ^= x >> 16, x *= 0x7feb352d, x ^= x >> 15, x *= 0x846ca68b,
+ * x ^= x >> 16: r = h mod 2^20 (m), h >> 11 (v).  A moment that is no number is held as zero (v: as the least value).
+ * The norm N of the last step lies in the workspace, at the byte offset that came_b200_plan_norm_offset gives (one fp32
+ * number; -1 when the plan takes none).
+ */
+int64_t came_b200_plan_norm_offset(const came_plan_t* plan);
+
+/*
+ * Norm of the gradients of many tensors, and clip by it (no counterpart in the reference): *norm (device memory) becomes
+ * N = sqrt(sum of all squares), then every gradient is multiplied by min(1, max_norm / (N + 1e-6)) in place (left alone where
+ * that is 1; with a N that is not a number all become NaN).  max_norm >= 0; infinity asks for the norm alone.  `grads`: host
+ * memory, read before the call returns; dense tensors of n elements each, in any order of dimensions, that do not overlap.
+ * workspace: came_b200_clip_workspace_bytes(n_tensors) bytes of device memory, 8-byte aligned, used until the call's kernels
+ * are done.  May be captured into a CUDA graph (addresses and max_norm are those of the capture).
+ */
+typedef struct CameGradRef {
+    void* g;
+    int64_t n;
+    int32_t dtype; /* CAME_DT_* */
+    int32_t reserved;
+} CameGradRef;
+size_t came_b200_clip_workspace_bytes(int n_tensors);
+int came_b200_clip_grad_norm(const CameGradRef* grads, int n_tensors, float max_norm, float* norm, void* workspace,
+                             size_t workspace_bytes, came_stream_t stream);
 
 /*
  * CUDA-graph capture.  came_b200_step may be called while `stream` is being captured: nothing in it synchronises
