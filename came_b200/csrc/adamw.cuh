@@ -2,8 +2,11 @@
 #pragma once
 
 #include "common.cuh"
+#include "launch.h"
 
 namespace came {
+
+constexpr int ADAMW_THREADS = 256;
 
 // ------------------------------------------------------------------------------------------
 // 8 consecutive elements <-> fp32 registers.  fp32: one 32-byte access; 16-bit types: one of 16 bytes.
@@ -28,9 +31,36 @@ __device__ __forceinline__ void store8(float* p, const float* v) {
 __device__ __forceinline__ void store8(__nv_bfloat16* p, const float* v) { store_run<8>(p, v); }
 __device__ __forceinline__ void store8(__half* p, const float* v) { store_run<8>(p, v); }
 
+__device__ __forceinline__ void load_words8(const uint32_t* p, uint32_t* w) {
+    asm volatile("ld.global.L1::no_allocate.v8.u32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                 : "l"(p) : "memory");
+}
+__device__ __forceinline__ uint2 load_words2(const void* p) {
+    uint2 r;
+    asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p) : "memory");
+    return r;
+}
+
 __device__ __forceinline__ float approx_sqrt(float x) {
     float y;
     asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// the same for arguments and results that are normal numbers (others become zero)
+__device__ __forceinline__ float fast_sqrt(float x) {
+    float y;
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float fast_rcp(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {      // (a NaN does not count)
+    float y;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
     return y;
 }
 
@@ -58,42 +88,27 @@ __device__ __forceinline__ float e8m0_inverse(uint32_t byte) { return __uint_as_
 template <int BITS>
 __device__ __forceinline__ float dither(float y, uint32_t r) { return __uint_as_float((__float_as_uint(y) + r) & ~((1u << BITS) - 1u)); }
 
-__device__ __forceinline__ void half2_floats(uint32_t w, float* v) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
-    v[0] = f.x;
-    v[1] = f.y;
+// two codes of a word of four (the lower or the upper two) <-> fp32
+__device__ __forceinline__ float2 e4m3_pair(uint32_t w, int upper) {
+    uint32_t h;
+    const uint16_t two = (uint16_t)(upper ? w >> 16 : w);
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(two));
+    return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
-__device__ __forceinline__ void e4m3_decode8(const uint2& c, float* v) {
-    const uint32_t w[2] = {c.x, c.y};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        uint32_t h;
-        const uint16_t two = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
-        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(two));
-        half2_floats(h, v + 2 * i);
-    }
+__device__ __forceinline__ float2 e5m2_pair(uint32_t w, int upper) {      // (e5m2 is the upper byte of fp16)
+    const uint32_t h = __byte_perm(w, 0u, upper ? 0x3424u : 0x1404u);
+    return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
-// e5m2 is the upper byte of fp16
-__device__ __forceinline__ void e5m2_decode8(const uint2& c, float* v) {
-    half2_floats(__byte_perm(c.x, 0u, 0x1404u), v);
-    half2_floats(__byte_perm(c.x, 0u, 0x3424u), v + 2);
-    half2_floats(__byte_perm(c.y, 0u, 0x1404u), v + 4);
-    half2_floats(__byte_perm(c.y, 0u, 0x3424u), v + 6);
+__device__ __forceinline__ uint32_t e4m3_codes(float lo, float hi) {
+    uint16_t c;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(c) : "f"(hi), "f"(lo));
+    return c;
 }
-__device__ __forceinline__ uint32_t e4m3_encode4(const float* v) {
-    uint16_t a, b;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(a) : "f"(v[1]), "f"(v[0]));
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(b) : "f"(v[3]), "f"(v[2]));
-    return (uint32_t)a | ((uint32_t)b << 16);
+__device__ __forceinline__ uint32_t e5m2_codes(float lo, float hi) {
+    uint16_t c;
+    asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(c) : "f"(hi), "f"(lo));
+    return c;
 }
-__device__ __forceinline__ uint32_t e5m2_encode4(const float* v) {
-    uint16_t a, b;
-    asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(a) : "f"(v[1]), "f"(v[0]));
-    asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(b) : "f"(v[3]), "f"(v[2]));
-    return (uint32_t)a | ((uint32_t)b << 16);
-}
-__device__ __forceinline__ uint2 e4m3_encode8(const float* v) { return make_uint2(e4m3_encode4(v), e4m3_encode4(v + 4)); }
-__device__ __forceinline__ uint2 e5m2_encode8(const float* v) { return make_uint2(e5m2_encode4(v), e5m2_encode4(v + 4)); }
 
 // ------------------------------------------------------------------------------------------
 // gradient norm: sums of squares per CTA in 64 bits, added in a fixed order by every CTA that needs the total
@@ -121,6 +136,90 @@ __device__ __forceinline__ double norm_of_partials(const double* parts, int n, d
 __device__ __forceinline__ double clip_coefficient(double norm, float max_norm) {
     const double c = (double)max_norm / (norm + 1e-6);
     return c > 1.0 ? 1.0 : c;      // (NaN stays)
+}
+
+// ------------------------------------------------------------------------------------------
+// what a warp needs of a tensor's step count and hyper-parameters
+// ------------------------------------------------------------------------------------------
+// What a tensor's step count and hyper-parameters make of the formulas
+struct AdamwCoef {
+    float c, b1, om1, b2, om2, size, root, eps, wd_lr;
+    uint32_t key;
+};
+
+// The same for a warp's tensors as long as count and group stay the same
+struct AdamwCache {
+    float step;
+    int group;
+    AdamwCoef k;
+};
+
+// 1 - beta^t, from ln beta as a sum of two fp32 numbers  (out of line: rare, and long)
+static __device__ __noinline__ double one_minus_power(float ln_hi, float ln_lo, double t) { return -expm1(t * ((double)ln_hi + (double)ln_lo)); }
+
+// (all lanes of a warp)
+__device__ __forceinline__ void adamw_coef(AdamwCache& cache, const CameTensorDesc& d, const CameHyper* hyp, bool clipped, double norm) {
+    const float step = *static_cast<const float*>(d.res_row);
+    if (step == cache.step && d.group == cache.group) return;      // (the same in every lane)
+    const CameHyper& h = hyp[d.group];
+    const double t = (double)step + 1.0;
+    // even lanes: lr / (1 - b1^t); odd lanes: 1 / sqrt(1 - b2^t)
+    const bool odd = threadIdx.x & 1;
+    const double rest = one_minus_power(odd ? h.om_beta3 : h.beta3, odd ? h.reserved[1] : h.reserved[0], t);
+    const float f = (float)(odd ? 1.0 / sqrt(rest) : (double)h.lr / rest);
+    cache.step = step;
+    cache.group = d.group;
+    AdamwCoef& k = cache.k;
+    k.size = __shfl_sync(0xffffffffu, f, 0);
+    k.root = __shfl_sync(0xffffffffu, f, 1);
+    k.c = clipped ? (float)((double)h.grad_scale * clip_coefficient(norm, h.clip_threshold)) : h.grad_scale;
+    k.b1 = h.beta1; k.om1 = h.om_beta1;
+    k.b2 = h.beta2; k.om2 = h.om_beta2;
+    k.eps = h.eps0; k.wd_lr = h.wd_lr;
+    k.key = mix32((uint32_t)t);
+}
+
+// The end of a launch: the last CTA raises the step counts of its tensors.  Every other CTA has read the counts it needs.
+__device__ __forceinline__ void adamw_count_step(const StepArgs& a, const AdamwArgs& w) {
+    __shared__ bool last;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        __threadfence();
+        last = atomicAdd(w.ticket, 1u) == gridDim.x - 1;
+    }
+    __syncthreads();
+    if (!last) return;
+    for (int i = threadIdx.x; i < w.n_tensors; i += ADAMW_THREADS) *static_cast<float*>(a.descs[w.tensors[i].tensor].res_row) += 1.0f;
+    if (threadIdx.x == 0) *w.ticket = 0u;
+}
+// The beginning: the norm of all gradients.  False: it is not finite, and the step does not take place.
+__device__ __forceinline__ bool adamw_norm(const AdamwArgs& w, double* norm) {
+    __shared__ double red[ADAMW_THREADS / 32];
+    *norm = 0.0;
+    if (!w.norm_parts) return true;
+    *norm = norm_of_partials(w.norm_parts, w.n_parts, red);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *w.norm_out = (float)*norm;
+    return isfinite(*norm);
+}
+
+// host side: pick the instance for a launch's types
+template <template <typename, typename> class Launch, typename P, typename... A>
+static cudaError_t adamw_for_g(int g_dtype, const A&... args) {
+    if (g_dtype == CAME_DT_F32) return Launch<P, float>::run(args...);
+    if (g_dtype == CAME_DT_F16) return Launch<P, __half>::run(args...);
+    return Launch<P, __nv_bfloat16>::run(args...);
+}
+template <template <typename, typename> class Launch, typename... A>
+static cudaError_t adamw_for(const KernelKey& key, const A&... args) {
+    if (key.p_dtype == CAME_DT_F32) return adamw_for_g<Launch, float>(key.g_dtype, args...);
+    if (key.p_dtype == CAME_DT_F16) return adamw_for_g<Launch, __half>(key.g_dtype, args...);
+    return adamw_for_g<Launch, __nv_bfloat16>(key.g_dtype, args...);
+}
+static AdamwHyp adamw_hyp(const CameHyper* host_hyp, int n_hyp) {
+    AdamwHyp h{};
+    if (host_hyp)
+        for (int i = 0; i < n_hyp && i < ADAMW_MAX_HYP; ++i) h.h[i] = host_hyp[i];
+    return h;
 }
 
 }  // namespace came

@@ -63,6 +63,12 @@ inline int elem_bytes(int dt) { return dt == CAME_DT_F32 ? 4 : 2; }
 inline bool is_adamw(const CameTensorDesc& d) { return d.mode == CAME_MODE_ADAMW || d.mode == CAME_MODE_ADAMW8; }
 inline bool is_nd(const CameTensorDesc& d) { return d.cols != 0 && d.batch > 1 && !is_adamw(d); }
 inline int64_t elements(const CameTensorDesc& d) { return d.rows * (d.cols ? d.cols : 1) * (d.batch > 1 ? (int64_t)d.batch : 1); }
+// (AdamW kernels copy from the 16-byte boundaries around an element)
+inline bool on_elements(const CameTensorDesc& d) {
+    auto on = [](const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % (uintptr_t)bytes == 0; };
+    const int state = d.mode == CAME_MODE_ADAMW ? 4 : 1;
+    return on(d.p, elem_bytes(d.p_dtype)) && on(d.g, elem_bytes(d.g_dtype)) && on(d.m, state) && on(d.sq_row, state) && on(d.res_row, 4);
+}
 inline int nd_chunk(const CameTensorDesc& d) { return is_nd(d) && !disable_fast() ? nd_small_batch(d.rows, d.cols) : 0; }
 
 // Which kernels take the passes of a matrix.
@@ -75,10 +81,10 @@ struct VecFlags {
 
 VecFlags vec_flags(const CameTensorDesc& d, bool fast) {
     VecFlags f{0, 0, 0};
-    if (is_adamw(d)) {      // eight elements of every tensor by one access of their own size each
+    if (is_adamw(d)) {      // eight elements of a tensor by one access
         auto on = [](const void* p, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; };
-        const uintptr_t state = d.mode == CAME_MODE_ADAMW ? 32 : 8;
-        f.v = on(d.p, 8 * elem_bytes(d.p_dtype)) && on(d.g, 8 * elem_bytes(d.g_dtype)) && on(d.m, state) && on(d.sq_row, state) ? 8 : 1;
+        if (d.mode == CAME_MODE_ADAMW8) f.v = on(d.m, 8) && on(d.sq_row, 8) ? 8 : 1;      // (parameters and gradients may start anywhere)
+        else f.v = on(d.p, 8 * elem_bytes(d.p_dtype)) && on(d.g, 8 * elem_bytes(d.g_dtype)) && on(d.m, 32) && on(d.sq_row, 32) ? 8 : 1;
         return f;
     }
     if (d.cols == 0 || is_nd(d)) return f;      // 1-D and N-D tensors have kernels of their own
@@ -123,14 +129,14 @@ int64_t generic_tiles(const CameTensorDesc& d, int bands) {
 size_t partial_floats(int64_t n) { return (size_t)(n + cdiv(n, PARTIAL_GROUP) + 1); }
 size_t partial_counters(int64_t n) { return (size_t)(1 + cdiv(n, PARTIAL_GROUP)); }
 
-// AdamW: 2048 elements (8 for each thread of a CTA) per item in small sets, so that all SMs have some; more where there are
-// items enough, so that a CTA sets up for more work.
+// AdamW: an item is a warp's.  256 elements in small sets, so that all SMs have some; up to 4096 where every resident warp
+// (24 per SM) still has four.
 int adamw_chunk(const CameTensorDesc* descs, int n) {
     double total = 0.0;
     for (int i = 0; i < n; ++i)
         if (is_adamw(descs[i])) total += (double)elements(descs[i]);
-    int chunk = 2048;
-    while (chunk < 16384 && total / chunk > 16.0 * 148) chunk *= 2;
+    int chunk = 256;
+    while (chunk < 4096 && total / chunk > 8.0 * 24 * 148) chunk *= 2;
     return chunk;
 }
 
@@ -290,6 +296,7 @@ int validate(const CameTensorDesc& d, int i) {
     if (is_adamw(d)) {
         if (!d.sq_row || !d.res_row) return fail(CAME_E_INVALID, "tensor %d: AdamW needs exp_avg_sq (sq_row) and a step count (res_row)", i);
         if (d.mode == CAME_MODE_ADAMW8 && (!d.m_absmax || !d.sq_row_absmax)) return fail(CAME_E_INVALID, "tensor %d: missing scales", i);
+        if (!on_elements(d)) return fail(CAME_E_INVALID, "tensor %d: p, g, fp32 states and the step count have to be aligned to their elements", i);
         const double n = (double)d.rows * (double)(d.cols ? d.cols : 1) * (double)(d.batch > 1 ? d.batch : 1);
         return n > 4.0e12 ? fail(CAME_E_UNSUPPORTED, "tensor %d: too many elements", i) : CAME_OK;      // (items are counted in 32 bits)
     }
@@ -850,6 +857,7 @@ int came_b200_plan_set_pointers(came_plan_t* plan, const void* const* g, void* c
         if (g) next.g = g[i];
         if (p) next.p = p[i];
         if (!next.g || !next.p) return fail(CAME_E_INVALID, "set_pointers: tensor %d: null pointer", i);
+        if (is_adamw(next) && !on_elements(next)) return fail(CAME_E_INVALID, "set_pointers: tensor %d: not aligned to its elements", i);
         if (!(vec_flags(next, fast) == plan->vflags[i]))
             return fail(CAME_E_INVALID, "set_pointers: tensor %d changes 16-byte alignment class; create a new plan", i);
         if (plan->n_push > 0 && plan->pushable[i] && pushed_param_in_range(*plan, plan->descs[i]) && !pushed_param_in_range(*plan, next))

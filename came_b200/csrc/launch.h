@@ -104,7 +104,7 @@ struct AdamwArgs {
     const Work* work;           // chunks of the tensors
     const Work* tensors;        // the tensors themselves, whose step counts the last CTA raises
     int n, n_tensors;
-    int chunk;                  // elements of an item (a multiple of 2048)
+    int chunk;                  // elements of an item (a multiple of 256)
     int by_value;
     uint32_t* ticket;           // CTAs that are through (zero between launches)
     const double* norm_parts;   // partial sums of the squared gradients, or null: no clip
@@ -112,6 +112,10 @@ struct AdamwArgs {
     int n_parts;
 };
 constexpr int ADAMW_MAX_HYP = 8;      // hyper-parameter records that travel as kernel arguments
+struct AdamwHyp {
+    CameHyper h[ADAMW_MAX_HYP];
+};
+cudaError_t launch_adamw8(const KernelKey& key, const StepArgs& a, const AdamwArgs& w, const AdamwHyp& h, cudaStream_t st);      // adamw8.cu
 cudaError_t launch_adamw(const KernelKey& key, const StepArgs& a, const AdamwArgs& w, const CameHyper* host_hyp, int n_hyp,
                          cudaStream_t st);
 // gradient norm (gradnorm.cu).  Sums of squares of the plan's AdamW gradients: parts[0 .. grad_norm_parts(n))
