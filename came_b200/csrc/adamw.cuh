@@ -1,12 +1,14 @@
 // Device helpers of the AdamW step and of the gradient norm.
 #pragma once
 
+#include <algorithm>
+
 #include "common.cuh"
 #include "launch.h"
 
 namespace came {
 
-constexpr int ADAMW_THREADS = 256;
+constexpr int ADAMW_THREADS = 256, ADAMW_WARPS = ADAMW_THREADS / 32;
 
 // ------------------------------------------------------------------------------------------
 // 8 consecutive elements <-> fp32 registers.  fp32: one 32-byte access; 16-bit types: one of 16 bytes.
@@ -200,6 +202,31 @@ __device__ __forceinline__ bool adamw_norm(const AdamwArgs& w, double* norm) {
     *norm = norm_of_partials(w.norm_parts, w.n_parts, red);
     if (blockIdx.x == 0 && threadIdx.x == 0) *w.norm_out = (float)*norm;
     return isfinite(*norm);
+}
+
+// A CTA takes spans of w.span consecutive items, one of every gridDim.x; items of a span that lie in one tensor are one run of
+// elements [lo, hi) of its n.
+template <typename F>
+__device__ __forceinline__ void for_runs(const StepArgs& a, const AdamwArgs& w, F f) {
+    for (int64_t from = (int64_t)blockIdx.x * w.span; from < w.n; from += (int64_t)gridDim.x * w.span) {
+        const int end = (int)min((int64_t)w.n, from + w.span);
+        for (int item = (int)from; item < end;) {
+            const Work wk = w.work[item];
+            const CameTensorDesc& d = a.descs[wk.tensor];
+            const int64_t n = d.rows * (d.cols ? d.cols : 1) * (d.batch > 1 ? (int64_t)d.batch : 1);
+            const int64_t lo = (int64_t)wk.tile * ADAMW_ITEM, hi = min(lo + (int64_t)(end - item) * ADAMW_ITEM, n);
+            item += (int)((hi - lo + ADAMW_ITEM - 1) / ADAMW_ITEM);
+            f(d, wk.tensor, lo, hi, n);
+        }
+    }
+}
+// Host side: the span and the grid.  Every CTA (per_sm on each SM) has the same number of spans, of `most` items at most: a span
+// in one piece spares the next run's set-up, but the shorter they are, the closer together lie the addresses that the GPU
+// works on at a time.
+static inline int adamw_spans(AdamwArgs& w, int per_sm, int most) {
+    const int64_t ctas = (int64_t)persistent_grid_limit() * per_sm, rounds = (w.n + ctas * most - 1) / (ctas * most);
+    w.span = (int)((w.n + ctas * rounds - 1) / (ctas * rounds));
+    return (int)std::min(ctas, ((int64_t)w.n + w.span - 1) / w.span);
 }
 
 // host side: pick the instance for a launch's types

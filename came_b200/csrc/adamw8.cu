@@ -17,15 +17,9 @@
 
 namespace came {
 
-#ifndef MINB
-#define MINB 2
-#endif
-#ifndef NST32
-#define NST32 4
-#endif
-#ifndef NST
-#define NST 4
-#endif
+// Two CTAs of 8 warps per SM and a ring of four slots: more warps mean fewer registers (80 at three CTAs: spills, 470 us where two
+// take 424 for 256 M bf16 elements), deeper rings bring nothing (five slots: 409 us, four: 406).
+constexpr int ADAMW8_CTAS = 2, ADAMW8_STAGES = 4;
 // A slot: 256 parameters and 256 gradients from the 32-byte boundary in front of them, then 16 bytes of codes (m, v) per lane.
 // A sector (32 bytes) of memory has to lie in one sector of the slot: split over two it is fetched twice (fp32: 36 instead of
 // 20 million sectors for 64 million elements, 940 instead of 640 us for 256 million).
@@ -33,16 +27,17 @@ constexpr float ADAMW8_TINY_EPS = 1e-16f;      // below it a root of less than 1
 template <typename P, typename G> struct Ring8 {
     static constexpr int G_OFF = QBLOCK * sizeof(P) + 32, MV_OFF = G_OFF + QBLOCK * sizeof(G) + 32;
     static constexpr int BYTES = MV_OFF + 32 * 16;
-    static constexpr int STAGES = sizeof(P) + sizeof(G) <= 4 ? NST : NST32;
+    static constexpr int STAGES = ADAMW8_STAGES;
     static constexpr int CTA_BYTES = BYTES * STAGES * (ADAMW_THREADS / 32);
 };
 
+constexpr int BSTEP = QBLOCK * ADAMW_WARPS;      // elements from a warp's block to its next one: the warps of a CTA take blocks in turn
 // The blocks a warp is at: addresses of this lane's 8 elements of the first one
 template <typename P, typename G> struct Span8 {
     P* p;
     const G* g;
     uint8_t *m, *v;
-    int64_t left;               // elements of the tensor from the span's first on
+    int64_t left;               // elements of the tensor from the first block on
     uint32_t p_off, g_off;      // bytes that the tensors start behind a 32-byte boundary
     int async_lo, async_hi;     // blocks that are copied asynchronously: all of them, and the boundaries around them, lie inside the tensor
 };
@@ -88,13 +83,13 @@ template <typename P, typename G>
 __device__ __forceinline__ void block8_fetch(uint8_t* slot, const Span8<P, G>& t, int b, int lane) {
     using R = Ring8<P, G>;
     if (b >= t.async_lo && b < t.async_hi) {
-        ring_copy<P>(slot, reinterpret_cast<const uint8_t*>(t.p + b * QBLOCK - 8 * lane) - t.p_off, t.p_off, lane);
-        ring_copy<G>(slot + R::G_OFF, reinterpret_cast<const uint8_t*>(t.g + b * QBLOCK - 8 * lane) - t.g_off, t.g_off, lane);
-        cp8(slot + R::MV_OFF + lane * 16, t.m + b * QBLOCK);
-        cp8(slot + R::MV_OFF + lane * 16 + 8, t.v + b * QBLOCK);
+        ring_copy<P>(slot, reinterpret_cast<const uint8_t*>(t.p + b * BSTEP - 8 * lane) - t.p_off, t.p_off, lane);
+        ring_copy<G>(slot + R::G_OFF, reinterpret_cast<const uint8_t*>(t.g + b * BSTEP - 8 * lane) - t.g_off, t.g_off, lane);
+        cp8(slot + R::MV_OFF + lane * 16, t.m + b * BSTEP);
+        cp8(slot + R::MV_OFF + lane * 16 + 8, t.v + b * BSTEP);
         return;
     }
-    const int at = b * QBLOCK, k = (int)max((int64_t)0, min((int64_t)8, t.left - at - 8 * lane));
+    const int at = b * BSTEP, k = (int)max((int64_t)0, min((int64_t)8, t.left - at - 8 * lane));
     ring_gather(slot, t.p + at, k, lane);
     ring_gather(slot + R::G_OFF, t.g + at, k, lane);
 #pragma unroll
@@ -166,15 +161,15 @@ template <typename P, typename G>
 __device__ __forceinline__ void block8_step(uint8_t* slot, const Span8<P, G>& t, int b, int lane, uint32_t group, uint32_t& ms, uint32_t& vs,
                                             const AdamwCoef& k) {
     using R = Ring8<P, G>;
-    const int at = b * QBLOCK;
+    const int at = b * BSTEP;
     const bool async = b >= t.async_lo && b < t.async_hi;
     uint32_t pw[2 * sizeof(P)], gw[2 * sizeof(G)];
     ring_read<G>(slot + R::G_OFF, async ? t.g_off : 0u, lane, gw);
     ring_read<P>(slot, async ? t.p_off : 0u, lane, pw);
     const uint4 codes = *reinterpret_cast<const uint4*>(slot + R::MV_OFF + lane * 16);
     Result8 r;
-    if (k.eps < ADAMW8_TINY_EPS) block8_math<P, G, true>(r, pw, gw, codes, ms, vs, group + 32u * b, k);
-    else block8_math<P, G, false>(r, pw, gw, codes, ms, vs, group + 32u * b, k);
+    if (k.eps < ADAMW8_TINY_EPS) block8_math<P, G, true>(r, pw, gw, codes, ms, vs, group + BSTEP / 8 * b, k);
+    else block8_math<P, G, false>(r, pw, gw, codes, ms, vs, group + BSTEP / 8 * b, k);
     ms = r.ms;
     vs = r.vs;
     if (async) {
@@ -214,12 +209,12 @@ __device__ __forceinline__ void span8_fast(uint8_t* ring, Span8<P, G> t, int n, 
     auto fetch = [&](int slot, int ahead) {      // the block `ahead` of the pointers
         uint8_t* to = ring + slot * R::BYTES;
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(P) / 2; ++i) cp16(to + 512 * i + 16 * lane, p_from + ahead * QBLOCK * (int)sizeof(P) + 512 * i, 16);
+        for (int i = 0; i < (int)sizeof(P) / 2; ++i) cp16(to + 512 * i + 16 * lane, p_from + ahead * BSTEP * (int)sizeof(P) + 512 * i, 16);
 #pragma unroll
         for (int i = 0; i < (int)sizeof(G) / 2; ++i)
-            cp16(to + R::G_OFF + 512 * i + 16 * lane, g_from + ahead * QBLOCK * (int)sizeof(G) + 512 * i, 16);
-        cp8(to + R::MV_OFF + lane * 16, m_from + ahead * QBLOCK);
-        cp8(to + R::MV_OFF + lane * 16 + 8, v_from + ahead * QBLOCK);
+            cp16(to + R::G_OFF + 512 * i + 16 * lane, g_from + ahead * BSTEP * (int)sizeof(G) + 512 * i, 16);
+        cp8(to + R::MV_OFF + lane * 16, m_from + ahead * BSTEP);
+        cp8(to + R::MV_OFF + lane * 16 + 8, v_from + ahead * BSTEP);
     };
 #pragma unroll
     for (int s = 0; s < S - 1; ++s) {
@@ -240,29 +235,29 @@ __device__ __forceinline__ void span8_fast(uint8_t* ring, Span8<P, G> t, int n, 
             ring_read<P>(slot, 0u, lane, pw);
             const uint4 codes = *reinterpret_cast<const uint4*>(slot + R::MV_OFF + lane * 16);
             Result8 r;
-            block8_math<P, G, false>(r, pw, gw, codes, __shfl_sync(0xffffffffu, ms, b + s), __shfl_sync(0xffffffffu, vs, b + s), group + 32u * s, k);
-            *reinterpret_cast<uint2*>(t.m + s * QBLOCK) = r.m;
-            *reinterpret_cast<uint2*>(t.v + s * QBLOCK) = r.v;
-            store8(t.p + s * QBLOCK, r.p);
+            block8_math<P, G, false>(r, pw, gw, codes, __shfl_sync(0xffffffffu, ms, b + s), __shfl_sync(0xffffffffu, vs, b + s), group + BSTEP / 8 * s, k);
+            *reinterpret_cast<uint2*>(t.m + s * BSTEP) = r.m;
+            *reinterpret_cast<uint2*>(t.v + s * BSTEP) = r.v;
+            store8(t.p + s * BSTEP, r.p);
             if (lane == b + s) {
                 ms = r.ms;
                 vs = r.vs;
             }
         }
-        p_from += S * QBLOCK * (int)sizeof(P);
-        g_from += S * QBLOCK * (int)sizeof(G);
-        m_from += S * QBLOCK;
-        v_from += S * QBLOCK;
-        t.p += S * QBLOCK;
-        t.m += S * QBLOCK;
-        t.v += S * QBLOCK;
-        group += 32u * S;
+        p_from += S * BSTEP * (int)sizeof(P);
+        g_from += S * BSTEP * (int)sizeof(G);
+        m_from += S * BSTEP;
+        v_from += S * BSTEP;
+        t.p += S * BSTEP;
+        t.m += S * BSTEP;
+        t.v += S * BSTEP;
+        group += BSTEP / 8 * S;
     }
     __syncwarp();
 }
 
 template <typename P, typename G>
-__global__ void __launch_bounds__(ADAMW_THREADS, MINB) k_adamw8(const StepArgs a, const AdamwArgs w, const __grid_constant__ AdamwHyp by_value) {
+__global__ void __launch_bounds__(ADAMW_THREADS, ADAMW8_CTAS) k_adamw8(const StepArgs a, const AdamwArgs w, const __grid_constant__ AdamwHyp by_value) {
     using R = Ring8<P, G>;
     extern __shared__ __align__(128) uint8_t ring_all[];
     const int lane = threadIdx.x & 31;
@@ -273,23 +268,21 @@ __global__ void __launch_bounds__(ADAMW_THREADS, MINB) k_adamw8(const StepArgs a
     AdamwCache cache;
     cache.step = -1.0f;
     cache.group = -1;
-    // an item (up to 32 blocks) is a warp's
-    for (int item = blockIdx.x + gridDim.x * (threadIdx.x >> 5); item < w.n; item += gridDim.x * (ADAMW_THREADS / 32)) {
-        const Work wk = w.work[item];
-        const CameTensorDesc& d = a.descs[wk.tensor];
-        const int64_t n = d.rows * (d.cols ? d.cols : 1) * (d.batch > 1 ? (int64_t)d.batch : 1);
-        const int64_t first = (int64_t)wk.tile * w.chunk / QBLOCK, at = first * QBLOCK + 8 * lane;
-        const int blocks = (int)(min((int64_t)w.chunk / QBLOCK, (n + QBLOCK - 1) / QBLOCK - first));
+    const int warp = threadIdx.x >> 5;
+    for_runs(a, w, [&](const CameTensorDesc& d, int tensor, int64_t lo, int64_t hi, int64_t n) {
+        const int64_t first = lo / QBLOCK + warp, at = first * QBLOCK + 8 * lane;
+        const int blocks = (int)((hi + QBLOCK - 1) / QBLOCK - first + ADAMW_WARPS - 1) / ADAMW_WARPS;      // this warp's
         uint8_t *m_scale = reinterpret_cast<uint8_t*>(d.m_absmax) + first, *v_scale = reinterpret_cast<uint8_t*>(d.sq_row_absmax) + first;
         Span8<P, G> t{static_cast<P*>(d.p) + at, static_cast<const G*>(d.g) + at, static_cast<uint8_t*>(d.m) + at, static_cast<uint8_t*>(d.sq_row) + at,
                       n - first * QBLOCK, (uint32_t)(reinterpret_cast<uintptr_t>(d.p) & 31u), (uint32_t)(reinterpret_cast<uintptr_t>(d.g) & 31u), 0, 0};
         const bool shifted = (t.p_off | t.g_off) != 0;
         t.async_lo = shifted && first == 0 ? 1 : 0;
-        if (a.scr[wk.tensor].g_v == 8) t.async_hi = (int)min((int64_t)blocks, (t.left - (shifted ? 8 : 0)) / QBLOCK);
-        uint32_t ms = 0u, vs = 0u;      // scale bytes of block `lane`
+        const int64_t sure = t.left - (shifted ? 8 : 0) - QBLOCK;      // the last place where a block can start
+        if (a.scr[tensor].g_v == 8 && sure >= 0) t.async_hi = (int)min((int64_t)blocks, sure / BSTEP + 1);
+        uint32_t ms = 0u, vs = 0u;      // scale bytes of the warp's block number `lane`
         if (lane < blocks) {
-            ms = m_scale[lane];
-            vs = v_scale[lane];
+            ms = m_scale[lane * ADAMW_WARPS];
+            vs = v_scale[lane * ADAMW_WARPS];
         }
         adamw_coef(cache, d, hyp, w.norm_parts != nullptr, norm);
         const uint32_t group = (uint32_t)(at >> 3);
@@ -322,10 +315,10 @@ __global__ void __launch_bounds__(ADAMW_THREADS, MINB) k_adamw8(const StepArgs a
         }
         __syncwarp();
         if (lane < blocks) {
-            m_scale[lane] = (uint8_t)ms;
-            v_scale[lane] = (uint8_t)vs;
+            m_scale[lane * ADAMW_WARPS] = (uint8_t)ms;
+            v_scale[lane * ADAMW_WARPS] = (uint8_t)vs;
         }
-    }
+    });
     adamw_count_step(a, w);
 }
 
@@ -334,7 +327,11 @@ template <typename P, typename G> struct LaunchAdamw8 {
         constexpr int smem = Ring8<P, G>::CTA_BYTES;
         const cudaError_t e = cudaFuncSetAttribute(k_adamw8<P, G>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e != cudaSuccess) return e;
-        k_adamw8<P, G><<<min(w.n, persistent_grid_limit() * MINB), ADAMW_THREADS, smem, st>>>(a, w, h);
+        // Spans (256 M elements): 16-bit types are bound by instructions, a long span fills its ring less often (406 us with 16
+        // items, 429 with 8, 511 with 4); fp32 is bound by DRAM, which likes addresses close together (682, 658, 641).
+        AdamwArgs x = w;
+        const int grid = adamw_spans(x, ADAMW8_CTAS, sizeof(P) + sizeof(G) <= 4 ? 16 : 4);
+        k_adamw8<P, G><<<grid, ADAMW_THREADS, smem, st>>>(a, x, h);
         return cudaGetLastError();
     }
 };

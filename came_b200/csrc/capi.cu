@@ -118,7 +118,6 @@ constexpr long long SMALL_SET_ELEMS = 16 << 20;
 struct Context {
     bool small;      // the whole-step kernel takes every matrix
     int bands;       // its bands of 16 rows per warp
-    int chunk;       // elements of an AdamW item
     bool generic(const CameTensorDesc& d) const { return d.cols != 0 && !is_nd(d) && !is_adamw(d) && (small || !vec_flags(d).wide); }
 };
 
@@ -129,17 +128,6 @@ int64_t generic_tiles(const CameTensorDesc& d, int bands) {
 size_t partial_floats(int64_t n) { return (size_t)(n + cdiv(n, PARTIAL_GROUP) + 1); }
 size_t partial_counters(int64_t n) { return (size_t)(1 + cdiv(n, PARTIAL_GROUP)); }
 
-// AdamW: an item is a warp's.  256 elements in small sets, so that all SMs have some; up to 4096 where every resident warp
-// (24 per SM) still has four.
-int adamw_chunk(const CameTensorDesc* descs, int n) {
-    double total = 0.0;
-    for (int i = 0; i < n; ++i)
-        if (is_adamw(descs[i])) total += (double)elements(descs[i]);
-    int chunk = 256;
-    while (chunk < 4096 && total / chunk > 8.0 * 24 * 148) chunk *= 2;
-    return chunk;
-}
-
 Context context(const CameTensorDesc* descs, int n) {
     const char* e = getenv("CAME_B200_SMALL_SET_ELEMS");
     const double line = e ? atof(e) : (double)SMALL_SET_ELEMS;
@@ -147,7 +135,7 @@ Context context(const CameTensorDesc* descs, int n) {
     for (int i = 0; i < n; ++i)
         if (vec_flags(descs[i]).wide)
             staged += (double)descs[i].rows * (double)descs[i].cols * (descs[i].mode == CAME_MODE_FLAT8 ? 4.0 / 3.0 : 1.0);
-    Context c{staged < line, 16, adamw_chunk(descs, n)};
+    Context c{staged < line, 16};
     auto items = [&](int bands) {
         int64_t tiles = 0;
         for (int i = 0; i < n; ++i)
@@ -181,7 +169,7 @@ Geometry geometry(const CameTensorDesc& d, const Context& ctx) {
     g.R = d.rows;
     g.C = d.cols;
     if (is_adamw(d)) {      // flat_chunks: items
-        g.flat_chunks = cdiv(elements(d), ctx.chunk);
+        g.flat_chunks = cdiv(elements(d), ADAMW_ITEM);
         return g;
     }
     g.nbR = (int)cdiv(g.R, QBLOCK);
@@ -417,7 +405,6 @@ struct came_plan {
     std::vector<char> pushable;    // ... or by the whole-step kernel, which serves the push mode too
     std::vector<char> push_must;   // pushable whatever the size of the set: has to lie in the local buffer (else it is not pushed)
     bool needs_hyp = false;        // some kernel reads the hyper-parameters from the workspace
-    int adamw_chunk = 0;
     bool adamw_clip = false;
     int norm_parts = 0;            // partial sums of the gradient norm
     int n_push = 0;                // push mode: peers that receive every parameter the fused kernel updates
@@ -614,7 +601,6 @@ int came_b200_plan_create(const CameTensorDesc* descs, int n_tensors, void* work
         std::map<Key, std::vector<int>> groups;
         for (int i = 0; i < n_tensors; ++i)
             if (is_adamw(D[i])) groups[Key{D[i].g_dtype, D[i].p_dtype, D[i].mode, 0}].push_back(i);
-        plan->adamw_chunk = ctx.chunk;
         plan->adamw_clip = n_clip > 0;
         const size_t first_item = work.size();
         if (plan->adamw_clip) plan->launches.push_back(LaunchItem{KID_GRAD_NORM, {}, first_item, 0, 0, 0, 0, 0, 0, 0, 0});
@@ -935,9 +921,9 @@ int came_b200_step(came_plan_t* plan, const CameHyper* hypers, int n_groups, cam
             cudaEventRecord(tm.t0, st);
         }
         if (it.kernel == KID_GRAD_NORM)
-            e = launch_grad_norm(a, wbase + it.work_off, it.n, plan->adamw_chunk, by_value ? norm : nullptr, n_groups, norm_parts, st);
+            e = launch_grad_norm(a, wbase + it.work_off, it.n, by_value ? norm : nullptr, n_groups, norm_parts, st);
         else if (it.kernel == KID_ADAMW || it.kernel == KID_ADAMW8) {
-            const AdamwArgs w{wbase + it.work_off, wbase + it.work2_off, it.n, it.n2, plan->adamw_chunk, 0,
+            const AdamwArgs w{wbase + it.work_off, wbase + it.work2_off, it.n, it.n2, 0, 0,
                               reinterpret_cast<uint32_t*>(plan->ws + plan->L.off_bar) + it.bar, plan->adamw_clip ? norm_parts : nullptr,
                               reinterpret_cast<float*>(plan->ws + plan->L.off_norm), plan->norm_parts};
             e = launch_adamw(it.key, a, w, by_value ? norm : nullptr, n_groups, st);

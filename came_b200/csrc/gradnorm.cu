@@ -70,33 +70,33 @@ __device__ __forceinline__ double chunk_squares_any(const void* g, int dtype, in
     return chunk_squares(static_cast<const __nv_bfloat16*>(g) + lo, n);
 }
 
-struct NormHyp {
-    CameHyper h[ADAMW_MAX_HYP];
-};
-__global__ void __launch_bounds__(NORM_THREADS) k_grad_norm(const StepArgs a, const Work* work, int n_work, int chunk, int use_value,
-                                                           const __grid_constant__ NormHyp by_value, double* parts) {
+__global__ void __launch_bounds__(NORM_THREADS) k_grad_norm(const StepArgs a, const AdamwArgs w, const __grid_constant__ AdamwHyp by_value,
+                                                           double* parts) {
     __shared__ double red[NORM_THREADS / 32];
-    const CameHyper* hyp = use_value ? by_value.h : a.hyp;
+    const CameHyper* hyp = w.by_value ? by_value.h : a.hyp;
     double t = 0.0;
-    for (int item = blockIdx.x; item < n_work; item += gridDim.x) {
-        const Work wk = work[item];
-        const CameTensorDesc& d = a.descs[wk.tensor];
-        const int64_t n = d.rows * (d.cols ? d.cols : 1) * (d.batch > 1 ? (int64_t)d.batch : 1), lo = (int64_t)wk.tile * chunk;
+    for_runs(a, w, [&](const CameTensorDesc& d, int, int64_t lo, int64_t hi, int64_t) {
         const double s = (double)hyp[d.group].grad_scale;
-        t += s * s * chunk_squares_any(d.g, d.g_dtype, lo, min((int64_t)chunk, n - lo));
-    }
+        t += s * s * chunk_squares_any(d.g, d.g_dtype, lo, hi - lo);
+    });
     t = block_sum64(t, red);
     if (threadIdx.x == 0) parts[blockIdx.x] = t;
 }
 
-int grad_norm_parts(int n) { return min(n, persistent_grid_limit() * NORM_CTAS); }
+static int norm_spans(AdamwArgs& w) { return adamw_spans(w, NORM_CTAS, 16); }
+int grad_norm_parts(int n) {
+    AdamwArgs w{};
+    w.n = n;
+    return norm_spans(w);
+}
 
-cudaError_t launch_grad_norm(const StepArgs& a, const Work* work, int n, int chunk, const CameHyper* host_hyp, int n_hyp, double* parts,
-                             cudaStream_t st) {
-    NormHyp h{};
-    if (host_hyp)
-        for (int i = 0; i < n_hyp && i < ADAMW_MAX_HYP; ++i) h.h[i] = host_hyp[i];
-    k_grad_norm<<<grad_norm_parts(n), NORM_THREADS, 0, st>>>(a, work, n, chunk, host_hyp != nullptr, h, parts);
+cudaError_t launch_grad_norm(const StepArgs& a, const Work* work, int n, const CameHyper* host_hyp, int n_hyp, double* parts, cudaStream_t st) {
+    AdamwArgs w{};
+    w.work = work;
+    w.n = n;
+    w.by_value = host_hyp != nullptr;
+    const int grid = norm_spans(w);
+    k_grad_norm<<<grid, NORM_THREADS, 0, st>>>(a, w, adamw_hyp(host_hyp, n_hyp), parts);
     return cudaGetLastError();
 }
 

@@ -104,13 +104,14 @@ struct AdamwArgs {
     const Work* work;           // chunks of the tensors
     const Work* tensors;        // the tensors themselves, whose step counts the last CTA raises
     int n, n_tensors;
-    int chunk;                  // elements of an item (a multiple of 256)
+    int span;                   // consecutive items that a CTA takes at a time (set by the launch)
     int by_value;
     uint32_t* ticket;           // CTAs that are through (zero between launches)
     const double* norm_parts;   // partial sums of the squared gradients, or null: no clip
     float* norm_out;
     int n_parts;
 };
+constexpr int ADAMW_ITEM = 2048;      // elements of a work item: 256 for each warp of a CTA
 constexpr int ADAMW_MAX_HYP = 8;      // hyper-parameter records that travel as kernel arguments
 struct AdamwHyp {
     CameHyper h[ADAMW_MAX_HYP];
@@ -120,7 +121,7 @@ cudaError_t launch_adamw(const KernelKey& key, const StepArgs& a, const AdamwArg
                          cudaStream_t st);
 // gradient norm (gradnorm.cu).  Sums of squares of the plan's AdamW gradients: parts[0 .. grad_norm_parts(n))
 int grad_norm_parts(int n);
-cudaError_t launch_grad_norm(const StepArgs& a, const Work* work, int n, int chunk, const CameHyper* host_hyp, int n_hyp, double* parts,
+cudaError_t launch_grad_norm(const StepArgs& a, const Work* work, int n, const CameHyper* host_hyp, int n_hyp, double* parts,
                              cudaStream_t st);
 // the same for tensors given by value, then (unless max_norm is infinite) their scaling in place
 size_t clip_parts(int n_tensors);      // doubles of workspace
