@@ -110,16 +110,16 @@ template <> __device__ __forceinline__ u64 word_pair<__half>(const uint32_t* w, 
 struct Result8 {
     float p[8];
     uint2 m, v;
-    uint32_t ms, vs;      // scale bytes
+    uint32_t m_top, v_top;      // bits of the block's largest magnitudes
 };
 
 // Elements go in pairs through the packed fp32 instructions.  Moments: every product and sum is rounded by itself, as separate
 // tensor operations round them, so that codes can be compared bit for bit (the scale is a power of two: scale * beta * code is
-// beta * value).  group: index of the 8 elements in their tensor.
+// beta * value).  m_keep, v_keep: beta * scale; group: index of the 8 elements in their tensor.
 template <typename P, typename G, bool TINY_EPS>
-__device__ __forceinline__ void block8_math(Result8& out, const uint32_t* pw, const uint32_t* gw, const uint4& codes, uint32_t ms, uint32_t vs,
+__device__ __forceinline__ void block8_math(Result8& out, const uint32_t* pw, const uint32_t* gw, const uint4& codes, float m_beta, float v_beta,
                                             uint32_t group, const AdamwCoef& k) {
-    const u64 m_keep = splat(k.b1 * e8m0_value(ms)), v_keep = splat(k.b2 * e8m0_value(vs));
+    const u64 m_keep = splat(m_beta), v_keep = splat(v_beta);
     const u64 c = splat(k.c), om1 = splat(k.om1), om2 = splat(k.om2);
     u64 m[4], v[4];
     float m_big = 0.0f, v_big = 0.0f;      // (a NaN does not count: it must not flush the rest of the block)
@@ -137,28 +137,51 @@ __device__ __forceinline__ void block8_math(Result8& out, const uint32_t* pw, co
         out.p[2 * j] = now.x;
         out.p[2 * j + 1] = now.y;
     }
-    out.ms = e8m0_scale<7>(__reduce_max_sync(0xffffffffu, __float_as_uint(m_big)));
-    const uint32_t v_top = __reduce_max_sync(0xffffffffu, __float_as_uint(v_big));
-    out.vs = e8m0_scale<14>(v_top);
-    const u64 m_inv = splat(e8m0_inverse(out.ms)), v_inv = splat(e8m0_inverse(out.vs));
-    // v > 0 stays above zero (its root divides); a block of zeros stays zero
-    const float least = v_top ? 0x1p-16f : 0.0f;
+    out.m_top = __reduce_max_sync(0xffffffffu, __float_as_uint(m_big));
+    out.v_top = __reduce_max_sync(0xffffffffu, __float_as_uint(v_big));
+    const u64 m_inv = splat(e8m0_inverse(e8m0_scale<7>(out.m_top)));
     const uint32_t h = mix32(group + k.key);
-    uint32_t mc[4], vc[4];
+    uint32_t r[8], mc[4], vc[4];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = h * (0x9E3779B1u * (2u * i + 1u));
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const uint32_t r0 = h * (0x9E3779B1u * (4u * j + 1u)), r1 = h * (0x9E3779B1u * (4u * j + 3u));
-        const u64 x = mul2(m[j], m_inv), y = mul2(v[j], v_inv);
-        mc[j] = e4m3_codes(dither<20>(x.x, r0 & 0xfffffu), dither<20>(x.y, r1 & 0xfffffu));
-        vc[j] = e5m2_codes(dither<21>(fmaxf(y.x, least), r0 >> 11), dither<21>(fmaxf(y.y, least), r1 >> 11));
+        const u64 x = mul2(m[j], m_inv);
+        mc[j] = e4m3_codes(dither<20>(x.x, r[2 * j] & 0xfffffu), dither<20>(x.y, r[2 * j + 1] & 0xfffffu));
+    }
+    // v stays above zero (its root divides): at least 2^-16 after scaling; a block of zeros stays zero
+    if (out.v_top >= 32u << 23) {
+        // The scale goes into the exponent with the random bits; what is less than 2^-16 then, or below zero (a v without an
+        // exponent of its own among them: its block's is 32 at least), is 2^-16 in one instruction.
+        const uint32_t shift = (141u << 23) - (out.v_top & 0x7f800000u);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int y0 = __viaddmax_s32(__float_as_int(v[j].x), (int)((r[2 * j] >> 11) + shift), 111 << 23);
+            const int y1 = __viaddmax_s32(__float_as_int(v[j].y), (int)((r[2 * j + 1] >> 11) + shift), 111 << 23);
+            vc[j] = e5m2_codes(__int_as_float(y0 & ~0x1fffff), __int_as_float(y1 & ~0x1fffff));
+        }
+    } else {
+        const u64 v_inv = splat(e8m0_inverse(e8m0_scale<14>(out.v_top)));
+        const float least = out.v_top ? 0x1p-16f : 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const u64 y = mul2(v[j], v_inv);
+            vc[j] = e5m2_codes(dither<21>(fmaxf(y.x, least), r[2 * j] >> 11), dither<21>(fmaxf(y.y, least), r[2 * j + 1] >> 11));
+        }
     }
     out.m = make_uint2(__byte_perm(mc[0], mc[1], 0x5410u), __byte_perm(mc[2], mc[3], 0x5410u));
     out.v = make_uint2(__byte_perm(vc[0], vc[1], 0x5410u), __byte_perm(vc[2], vc[3], 0x5410u));
 }
 
-// A block of any kind: scale bytes ms, vs in and out
+// Scales of a warp's blocks: lane l holds those of block l
+struct Scales8 {
+    float m_beta, v_beta;       // old: beta * scale
+    uint32_t m_top, v_top;      // new: bits of the largest magnitudes
+};
+
+// A block of any kind
 template <typename P, typename G>
-__device__ __forceinline__ void block8_step(uint8_t* slot, const Span8<P, G>& t, int b, int lane, uint32_t group, uint32_t& ms, uint32_t& vs,
+__device__ __forceinline__ void block8_step(uint8_t* slot, const Span8<P, G>& t, int b, int lane, uint32_t group, Scales8& sc,
                                             const AdamwCoef& k) {
     using R = Ring8<P, G>;
     const int at = b * BSTEP;
@@ -168,10 +191,13 @@ __device__ __forceinline__ void block8_step(uint8_t* slot, const Span8<P, G>& t,
     ring_read<P>(slot, async ? t.p_off : 0u, lane, pw);
     const uint4 codes = *reinterpret_cast<const uint4*>(slot + R::MV_OFF + lane * 16);
     Result8 r;
-    if (k.eps < ADAMW8_TINY_EPS) block8_math<P, G, true>(r, pw, gw, codes, ms, vs, group + BSTEP / 8 * b, k);
-    else block8_math<P, G, false>(r, pw, gw, codes, ms, vs, group + BSTEP / 8 * b, k);
-    ms = r.ms;
-    vs = r.vs;
+    const float m_beta = __shfl_sync(0xffffffffu, sc.m_beta, b), v_beta = __shfl_sync(0xffffffffu, sc.v_beta, b);
+    if (k.eps < ADAMW8_TINY_EPS) block8_math<P, G, true>(r, pw, gw, codes, m_beta, v_beta, group + BSTEP / 8 * b, k);
+    else block8_math<P, G, false>(r, pw, gw, codes, m_beta, v_beta, group + BSTEP / 8 * b, k);
+    if (lane == b) {
+        sc.m_top = r.m_top;
+        sc.v_top = r.v_top;
+    }
     if (async) {
         *reinterpret_cast<uint2*>(t.m + at) = r.m;
         *reinterpret_cast<uint2*>(t.v + at) = r.v;
@@ -200,7 +226,7 @@ __device__ __forceinline__ void block8_step(uint8_t* slot, const Span8<P, G>& t,
 // Whole blocks of tensors on 32-byte boundaries, STAGES of them at a time (n a multiple of that): every place in the ring is
 // known when this is compiled, and nothing is asked per block.  Returns with the ring empty.
 template <typename P, typename G>
-__device__ __forceinline__ void span8_fast(uint8_t* ring, Span8<P, G> t, int n, int lane, uint32_t group, uint32_t& ms, uint32_t& vs,
+__device__ __forceinline__ void span8_fast(uint8_t* ring, Span8<P, G> t, int n, int lane, uint32_t group, Scales8& sc,
                                            const AdamwCoef& k) {
     using R = Ring8<P, G>;
     constexpr int S = R::STAGES;
@@ -235,13 +261,14 @@ __device__ __forceinline__ void span8_fast(uint8_t* ring, Span8<P, G> t, int n, 
             ring_read<P>(slot, 0u, lane, pw);
             const uint4 codes = *reinterpret_cast<const uint4*>(slot + R::MV_OFF + lane * 16);
             Result8 r;
-            block8_math<P, G, false>(r, pw, gw, codes, __shfl_sync(0xffffffffu, ms, b + s), __shfl_sync(0xffffffffu, vs, b + s), group + BSTEP / 8 * s, k);
+            block8_math<P, G, false>(r, pw, gw, codes, __shfl_sync(0xffffffffu, sc.m_beta, b + s), __shfl_sync(0xffffffffu, sc.v_beta, b + s),
+                                     group + BSTEP / 8 * s, k);
             *reinterpret_cast<uint2*>(t.m + s * BSTEP) = r.m;
             *reinterpret_cast<uint2*>(t.v + s * BSTEP) = r.v;
             store8(t.p + s * BSTEP, r.p);
             if (lane == b + s) {
-                ms = r.ms;
-                vs = r.vs;
+                sc.m_top = r.m_top;
+                sc.v_top = r.v_top;
             }
         }
         p_from += S * BSTEP * (int)sizeof(P);
@@ -279,17 +306,18 @@ __global__ void __launch_bounds__(ADAMW_THREADS, ADAMW8_CTAS) k_adamw8(const Ste
         t.async_lo = shifted && first == 0 ? 1 : 0;
         const int64_t sure = t.left - (shifted ? 8 : 0) - QBLOCK;      // the last place where a block can start
         if (a.scr[tensor].g_v == 8 && sure >= 0) t.async_hi = (int)min((int64_t)blocks, sure / BSTEP + 1);
-        uint32_t ms = 0u, vs = 0u;      // scale bytes of the warp's block number `lane`
+        uint32_t ms = 0u, vs = 0u;
         if (lane < blocks) {
             ms = m_scale[lane * ADAMW_WARPS];
             vs = v_scale[lane * ADAMW_WARPS];
         }
         adamw_coef(cache, d, hyp, w.norm_parts != nullptr, norm);
+        Scales8 sc{cache.k.b1 * e8m0_value(ms), cache.k.b2 * e8m0_value(vs), 0u, 0u};
         const uint32_t group = (uint32_t)(at >> 3);
         int b = 0;
         if (!shifted && cache.k.eps >= ADAMW8_TINY_EPS && t.async_hi >= R::STAGES) {
             b = t.async_hi / R::STAGES * R::STAGES;
-            span8_fast(ring, t, b, lane, group, ms, vs, cache.k);
+            span8_fast(ring, t, b, lane, group, sc, cache.k);
         }
 #pragma unroll
         for (int s = 0; s < R::STAGES - 1; ++s) {
@@ -304,19 +332,14 @@ __global__ void __launch_bounds__(ADAMW_THREADS, ADAMW8_CTAS) k_adamw8(const Ste
             cp_commit();
             cp_wait<R::STAGES - 1>();
             __syncwarp();
-            uint32_t m_byte = __shfl_sync(0xffffffffu, ms, b), v_byte = __shfl_sync(0xffffffffu, vs, b);
-            block8_step(slot, t, b, lane, group, m_byte, v_byte, cache.k);
-            if (lane == b) {
-                ms = m_byte;
-                vs = v_byte;
-            }
+            block8_step(slot, t, b, lane, group, sc, cache.k);
             ahead = slot;
             slot = slot == ring + (R::STAGES - 1) * R::BYTES ? ring : slot + R::BYTES;
         }
         __syncwarp();
         if (lane < blocks) {
-            m_scale[lane * ADAMW_WARPS] = (uint8_t)ms;
-            v_scale[lane * ADAMW_WARPS] = (uint8_t)vs;
+            m_scale[lane * ADAMW_WARPS] = (uint8_t)e8m0_scale<7>(sc.m_top);
+            v_scale[lane * ADAMW_WARPS] = (uint8_t)e8m0_scale<14>(sc.v_top);
         }
     });
     adamw_count_step(a, w);
