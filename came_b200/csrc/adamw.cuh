@@ -181,8 +181,9 @@ __device__ __forceinline__ void adamw_coef(AdamwCache& cache, const CameTensorDe
     k.key = mix32((uint32_t)t);
 }
 
-// The end of a launch: the last CTA raises the step counts of its tensors.  Every other CTA has read the counts it needs.
-__device__ __forceinline__ void adamw_count_step(const StepArgs& a, const AdamwArgs& w) {
+// The end of a CTA: the last one raises the step counts of the launch's tensors.  Every warp of every CTA has read the counts it
+// needs by then.
+__device__ __forceinline__ void adamw_count_step(const AdamwArgs& w) {
     __shared__ bool last;
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -191,8 +192,27 @@ __device__ __forceinline__ void adamw_count_step(const StepArgs& a, const AdamwA
     }
     __syncthreads();
     if (!last) return;
-    for (int i = threadIdx.x; i < w.n_tensors; i += ADAMW_THREADS) *static_cast<float*>(a.descs[w.tensors[i].tensor].res_row) += 1.0f;
+    for (int i = threadIdx.x; i < w.n_tensors; i += ADAMW_THREADS) atomicAdd(w.steps[i], 1.0f);      // (one address each: nothing to wait for)
     if (threadIdx.x == 0) *w.ticket = 0u;
+}
+// Launches that may begin while the one before them on the stream ends: after griddep_launch() of all its CTAs, which comes when a
+// CTA has no more runs (earlier, the waiting CTAs would spread unevenly over the SMs: 1 % of a large step).  It is the end of
+// that launch that griddep_wait() waits for; nothing in memory is touched before.
+__device__ __forceinline__ void griddep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void griddep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+template <typename... P, typename... A>
+static cudaError_t launch_behind(void (*kernel)(P...), int grid, int threads, int smem, cudaStream_t st, const A&... args) {
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t c{};
+    c.gridDim = dim3((unsigned)grid);
+    c.blockDim = dim3((unsigned)threads);
+    c.dynamicSmemBytes = (size_t)smem;
+    c.stream = st;
+    c.attrs = &early;
+    c.numAttrs = 1;
+    return cudaLaunchKernelEx(&c, kernel, args...);
 }
 // The beginning: the norm of all gradients.  False: it is not finite, and the step does not take place.
 __device__ __forceinline__ bool adamw_norm(const AdamwArgs& w, double* norm) {

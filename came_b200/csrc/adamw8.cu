@@ -23,7 +23,9 @@ constexpr int ADAMW8_CTAS = 2, ADAMW8_STAGES = 4;
 // A slot: 256 parameters and 256 gradients from the 32-byte boundary in front of them, then 16 bytes of codes (m, v) per lane.
 // A sector (32 bytes) of memory has to lie in one sector of the slot: split over two it is fetched twice (fp32: 36 instead of
 // 20 million sectors for 64 million elements, 940 instead of 640 us for 256 million).
-constexpr float ADAMW8_TINY_EPS = 1e-16f;      // below it a root of less than 1e-19, which the fast one takes for zero, would count
+// The fast root takes what is below 1.2e-38 for zero, the true one 1.1e-19 at most: with eps 2^24 times that (times the factor of
+// the root) or more, no digit of their sum is lost.
+constexpr float ADAMW8_LOST_ROOT = 2e-12f;
 template <typename P, typename G> struct Ring8 {
     static constexpr int G_OFF = QBLOCK * sizeof(P) + 32, MV_OFF = G_OFF + QBLOCK * sizeof(G) + 32;
     static constexpr int BYTES = MV_OFF + 32 * 16;
@@ -192,7 +194,7 @@ __device__ __forceinline__ void block8_step(uint8_t* slot, const Span8<P, G>& t,
     const uint4 codes = *reinterpret_cast<const uint4*>(slot + R::MV_OFF + lane * 16);
     Result8 r;
     const float m_beta = __shfl_sync(0xffffffffu, sc.m_beta, b), v_beta = __shfl_sync(0xffffffffu, sc.v_beta, b);
-    if (k.eps < ADAMW8_TINY_EPS) block8_math<P, G, true>(r, pw, gw, codes, m_beta, v_beta, group + BSTEP / 8 * b, k);
+    if (k.eps < ADAMW8_LOST_ROOT * k.root) block8_math<P, G, true>(r, pw, gw, codes, m_beta, v_beta, group + BSTEP / 8 * b, k);
     else block8_math<P, G, false>(r, pw, gw, codes, m_beta, v_beta, group + BSTEP / 8 * b, k);
     if (lane == b) {
         sc.m_top = r.m_top;
@@ -290,6 +292,7 @@ __global__ void __launch_bounds__(ADAMW_THREADS, ADAMW8_CTAS) k_adamw8(const Ste
     const int lane = threadIdx.x & 31;
     uint8_t* ring = ring_all + (threadIdx.x >> 5) * (R::BYTES * R::STAGES);
     const CameHyper* hyp = w.by_value ? by_value.h : a.hyp;
+    griddep_wait();
     double norm;
     if (!adamw_norm(w, &norm)) return;      // (in every CTA, and before anything is written)
     AdamwCache cache;
@@ -315,7 +318,7 @@ __global__ void __launch_bounds__(ADAMW_THREADS, ADAMW8_CTAS) k_adamw8(const Ste
         Scales8 sc{cache.k.b1 * e8m0_value(ms), cache.k.b2 * e8m0_value(vs), 0u, 0u};
         const uint32_t group = (uint32_t)(at >> 3);
         int b = 0;
-        if (!shifted && cache.k.eps >= ADAMW8_TINY_EPS && t.async_hi >= R::STAGES) {
+        if (!shifted && cache.k.eps >= ADAMW8_LOST_ROOT * cache.k.root && t.async_hi >= R::STAGES) {
             b = t.async_hi / R::STAGES * R::STAGES;
             span8_fast(ring, t, b, lane, group, sc, cache.k);
         }
@@ -342,7 +345,8 @@ __global__ void __launch_bounds__(ADAMW_THREADS, ADAMW8_CTAS) k_adamw8(const Ste
             v_scale[lane * ADAMW_WARPS] = (uint8_t)e8m0_scale<14>(sc.v_top);
         }
     });
-    adamw_count_step(a, w);
+    griddep_launch();
+    adamw_count_step(w);
 }
 
 template <typename P, typename G> struct LaunchAdamw8 {
@@ -354,8 +358,7 @@ template <typename P, typename G> struct LaunchAdamw8 {
         // items, 429 with 8, 511 with 4); fp32 is bound by DRAM, which likes addresses close together (682, 658, 641).
         AdamwArgs x = w;
         const int grid = adamw_spans(x, ADAMW8_CTAS, sizeof(P) + sizeof(G) <= 4 ? 16 : 4);
-        k_adamw8<P, G><<<grid, ADAMW_THREADS, smem, st>>>(a, x, h);
-        return cudaGetLastError();
+        return launch_behind(k_adamw8<P, G>, grid, ADAMW_THREADS, smem, st, a, x, h);
     }
 };
 

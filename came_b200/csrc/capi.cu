@@ -625,7 +625,12 @@ int came_b200_plan_create(const CameTensorDesc* descs, int n_tensors, void* work
             LaunchItem& it = plan->launches[k++];
             it.work2_off = work.size();
             it.n2 = (int)kv.second.size();
-            for (int i : kv.second) work.push_back(Work{i, 0});
+            for (int i : kv.second) {      // addresses of the step counts, in entries of the same size
+                Work entry;
+                static_assert(sizeof(Work) == sizeof(void*), "an entry holds a pointer");
+                std::memcpy(&entry, &D[i].res_row, sizeof(entry));
+                work.push_back(entry);
+            }
         }
     }
     // tensors of more than two dimensions
@@ -923,7 +928,7 @@ int came_b200_step(came_plan_t* plan, const CameHyper* hypers, int n_groups, cam
         if (it.kernel == KID_GRAD_NORM)
             e = launch_grad_norm(a, wbase + it.work_off, it.n, by_value ? norm : nullptr, n_groups, norm_parts, st);
         else if (it.kernel == KID_ADAMW || it.kernel == KID_ADAMW8) {
-            const AdamwArgs w{wbase + it.work_off, wbase + it.work2_off, it.n, it.n2, 0, 0,
+            const AdamwArgs w{wbase + it.work_off, reinterpret_cast<float* const*>(wbase + it.work2_off), it.n, it.n2, 0, 0,
                               reinterpret_cast<uint32_t*>(plan->ws + plan->L.off_bar) + it.bar, plan->adamw_clip ? norm_parts : nullptr,
                               reinterpret_cast<float*>(plan->ws + plan->L.off_norm), plan->norm_parts};
             e = launch_adamw(it.key, a, w, by_value ? norm : nullptr, n_groups, st);

@@ -74,11 +74,13 @@ __global__ void __launch_bounds__(NORM_THREADS) k_grad_norm(const StepArgs a, co
                                                            double* parts) {
     __shared__ double red[NORM_THREADS / 32];
     const CameHyper* hyp = w.by_value ? by_value.h : a.hyp;
+    griddep_wait();
     double t = 0.0;
     for_runs(a, w, [&](const CameTensorDesc& d, int, int64_t lo, int64_t hi, int64_t) {
         const double s = (double)hyp[d.group].grad_scale;
         t += s * s * chunk_squares_any(d.g, d.g_dtype, lo, hi - lo);
     });
+    griddep_launch();
     t = block_sum64(t, red);
     if (threadIdx.x == 0) parts[blockIdx.x] = t;
 }
@@ -96,8 +98,7 @@ cudaError_t launch_grad_norm(const StepArgs& a, const Work* work, int n, const C
     w.n = n;
     w.by_value = host_hyp != nullptr;
     const int grid = norm_spans(w);
-    k_grad_norm<<<grid, NORM_THREADS, 0, st>>>(a, w, adamw_hyp(host_hyp, n_hyp), parts);
-    return cudaGetLastError();
+    return launch_behind(k_grad_norm, grid, NORM_THREADS, 0, st, a, w, adamw_hyp(host_hyp, n_hyp), parts);
 }
 
 // ---- tensors given by value: the table is a kernel argument (the limit is 32 764 bytes), nothing is uploaded -------------
@@ -124,12 +125,14 @@ __device__ __forceinline__ int tensor_of(const GradTable<N>& t, int c) {
 template <int N>
 __global__ void __launch_bounds__(NORM_THREADS) k_clip_norm(const __grid_constant__ GradTable<N> t, double* parts) {
     __shared__ double red[NORM_THREADS / 32];
+    griddep_wait();
     double s = 0.0;
     for (int c = blockIdx.x; c < t.first[t.count]; c += gridDim.x) {
         const int i = tensor_of(t, c);
         const int64_t lo = (int64_t)(c - t.first[i]) * t.chunk;
         s += chunk_squares_any(t.g[i], t.dtype[i], lo, min((int64_t)t.chunk, t.n[i] - lo));
     }
+    griddep_launch();
     s = block_sum64(s, red);
     if (threadIdx.x == 0) parts[blockIdx.x] = s;
 }
@@ -151,6 +154,7 @@ template <int N>
 __global__ void __launch_bounds__(NORM_THREADS) k_clip_scale(const __grid_constant__ GradTable<N> t, const double* parts, int n_parts,
                                                             float max_norm, float* norm_out) {
     __shared__ double red[NORM_THREADS / 32];
+    griddep_wait();
     const double norm = norm_of_partials(parts, n_parts, red);
     if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
     const float c = (float)clip_coefficient(norm, max_norm);
@@ -190,12 +194,10 @@ static cudaError_t clip_pass(const CameGradRef* grads, int n, int chunk, bool sc
                              float* norm, cudaStream_t st) {
     const GradTable<N> t = clip_table<N>(grads, n, chunk);
     const int grid = clip_grid(t.first[n]);
-    if (scale) k_clip_scale<N><<<grid, NORM_THREADS, 0, st>>>(t, parts, *n_parts, max_norm, norm);
-    else {
-        k_clip_norm<N><<<grid, NORM_THREADS, 0, st>>>(t, parts + *n_parts);
-        *n_parts += grid;
-    }
-    return cudaGetLastError();
+    if (scale) return launch_behind(k_clip_scale<N>, grid, NORM_THREADS, 0, st, t, static_cast<const double*>(parts), *n_parts, max_norm, norm);
+    double* const to = parts + *n_parts;
+    *n_parts += grid;
+    return launch_behind(k_clip_norm<N>, grid, NORM_THREADS, 0, st, t, to);
 }
 
 cudaError_t launch_clip(const CameGradRef* grads, int n, float max_norm, float* norm, double* parts, cudaStream_t st) {
@@ -217,8 +219,7 @@ cudaError_t launch_clip(const CameGradRef* grads, int n, float max_norm, float* 
         }
     if (e == cudaSuccess && (norm_only || n == 0)) {      // the total alone: an empty table
         const GradTable<CLIP_FEW> none{};
-        k_clip_scale<CLIP_FEW><<<1, NORM_THREADS, 0, st>>>(none, parts, n_parts, max_norm, norm);
-        e = cudaGetLastError();
+        e = launch_behind(k_clip_scale<CLIP_FEW>, 1, NORM_THREADS, 0, st, none, static_cast<const double*>(parts), n_parts, max_norm, norm);
     }
     return e;
 }

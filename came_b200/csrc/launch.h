@@ -102,7 +102,7 @@ cudaError_t launch_nd_fixed(int kernel, const KernelKey& key, const StepArgs& a,
 // AdamW (adamw.cu): one launch per (gradient type, parameter type, layout)
 struct AdamwArgs {
     const Work* work;           // chunks of the tensors
-    const Work* tensors;        // the tensors themselves, whose step counts the last CTA raises
+    float* const* steps;        // the tensors' step counts, which the last CTA raises
     int n, n_tensors;
     int span;                   // consecutive items that a CTA takes at a time (set by the launch)
     int by_value;

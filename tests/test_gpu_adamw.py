@@ -83,6 +83,7 @@ def _check_step(opt, step, c=1.0, c_err=0.0, hyper=None):
         p64, upd = ref.param(old.double(), m64, v64, t + 1, wd=group["weight_decay"], **h)
         # (a moment that is almost nothing of its two terms: its own bound instead of one relative to it)
         slack = h["lr"] / (1 - h["betas"][0] ** (t + 1)) * m_tol / (v64.sqrt() / (1 - h["betas"][1] ** (t + 1)) ** 0.5 + h["eps"])
+        slack = slack + upd.abs() * 1e-44 / v64.clamp(min=1e-60)      # (a v next to nothing: its last bit is more than a rounding)
         err, tol = (p.detach().double() - p64).abs(), ref.param_bound(p64, upd, p.dtype) + (1.02 + 4 * c_err) * slack + c_err * upd.abs()
         tol = torch.where(torch.isfinite(tol), tol, torch.zeros_like(tol))
         assert (err <= tol).all(), (tuple(p.shape), (err - tol).max().item())
@@ -157,6 +158,18 @@ def test_gradient_ranges(kind, scale):
     if scale == 0.0:
         st = opt.state[ps[0]]
         assert not any(v.float().any() for key, v in st.items() if key in ("exp_avg", "exp_avg_sq", "exp_avg_q", "exp_avg_sq_q"))
+
+
+@pytest.mark.parametrize("kind", ["fp32", "8bit"])
+@pytest.mark.parametrize("eps", [1e-20, 1e-15, 1e-11, 1e-9])
+def test_second_moments_next_to_nothing(kind, eps):
+    """Roots of numbers at the lower end of fp32 beside an eps of their size."""
+    ps = _params([(1000,), (64, 96)], torch.float32)
+    opt = _cls(kind)(ps, **{**HYPER, "eps": eps, "betas": (0.9, 0.9999)})
+    for k in range(3):
+        _set_grads(ps, k, 3e-17)
+        ps[1].grad *= 10.0 ** torch.arange(-2, 4, device="cuda").repeat(16)
+        _check_step(opt, opt.step)
 
 
 def test_agrees_with_torch_and_loads_its_checkpoint():
