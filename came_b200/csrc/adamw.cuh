@@ -33,17 +33,6 @@ __device__ __forceinline__ void store8(float* p, const float* v) {
 __device__ __forceinline__ void store8(__nv_bfloat16* p, const float* v) { store_run<8>(p, v); }
 __device__ __forceinline__ void store8(__half* p, const float* v) { store_run<8>(p, v); }
 
-__device__ __forceinline__ void load_words8(const uint32_t* p, uint32_t* w) {
-    asm volatile("ld.global.L1::no_allocate.v8.u32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
-                 : "l"(p) : "memory");
-}
-__device__ __forceinline__ uint2 load_words2(const void* p) {
-    uint2 r;
-    asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p) : "memory");
-    return r;
-}
-
 __device__ __forceinline__ float approx_sqrt(float x) {
     float y;
     asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -132,6 +132,31 @@ def test_steps_follow_the_definition(kind, dtype, packed):
         assert all(torch.equal(p.grad, g) for p, g in zip(ps, gs) if p.grad is not None)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("packed", [False, True])
+def test_codes_equal_those_of_separate_fp32_operations(dtype, packed):
+    """Moments formed by one tensor operation per product and sum, rounded by the oracle: the same bytes, at any scale."""
+    ps = _params([(70000,), (129, 1026), (257,), (64, 4096), (9000,)], dtype, packed=packed)
+    opt = _cls("8bit")(ps, lr=1e-3, betas=(0.9, 0.99))
+    opt.param_groups[0]["grad_scale"] = 0.125
+    for k, scale in enumerate((1e-2, 1e-2, 1e-5, 1e-3, 1.0)):
+        _set_grads(ps, k, scale, packed)
+        if dtype == torch.float32 and k == 3:      # blocks next to underflow, some of them zero
+            ps[0].grad *= 10.0 ** -torch.arange(0, 40, 4, device="cuda").repeat_interleave(7000)
+            ps[2].grad[:] = 0.0
+        before = {p: _state(opt, p) for p in ps}
+        opt.step()
+        for p in ps:
+            m, v, t = before[p]
+            g = p.grad.float() * 0.125
+            m, v = m.float() * 0.9 + g * (1.0 - 0.9), v.float() * 0.99 + g * g * (1.0 - 0.99)
+            st = opt.state[p]
+            for x, which, key in ((m, "m", "exp_avg"), (v, "v", "exp_avg_sq")):
+                codes, scales = ref.encode(x, which, t + 1)
+                assert torch.equal(scales, st[key + "_scale"].float())
+                assert torch.equal(codes.view(torch.uint8), st[key + "_q"].view(torch.uint8)), (tuple(p.shape), which, k)
+
+
 @pytest.mark.parametrize("hyper", [dict(betas=(0.0, 0.0)), dict(betas=(0.0, 0.95)), dict(betas=(0.95, 0.5), eps=1.0), dict(lr=0.0),
                                    dict(weight_decay=0.0), dict(betas=(0.9, 0.99999), lr=1.0), dict(eps=1e-20, weight_decay=0.5)])
 @pytest.mark.parametrize("kind", ["fp32", "8bit"])
@@ -235,10 +260,11 @@ def test_strides(kind):
     assert torch.equal(wide[:, :3], keep[:, :3]) and torch.equal(wide[:, 40:], keep[:, 40:])
 
 
+@pytest.mark.parametrize("offset", [0, 4, 8])
 @pytest.mark.parametrize("kind", ["fp32", "8bit"])
-def test_nothing_beyond_the_tensor_is_written(kind):
-    """Sentinels on both sides of parameters and states."""
-    n = 1000 + 13
+def test_nothing_beyond_the_tensor_is_written(kind, offset):
+    """Sentinels on both sides of parameters and states, states off their boundaries."""
+    n = 3000 + 13
     buf = torch.full((n + 64,), 5.0, device="cuda", dtype=torch.bfloat16)
     p = torch.nn.Parameter(buf[32: 32 + n])
     p.grad = torch.ones_like(p)
@@ -247,17 +273,17 @@ def test_nothing_beyond_the_tensor_is_written(kind):
     st, around = opt.state[p], []
     for key in [k for k in st if k != "step"]:
         raw = torch.full((st[key].numel() * st[key].element_size() + 1024,), 77, device="cuda", dtype=torch.uint8)
-        mid = raw[512: 512 + st[key].numel() * st[key].element_size()]
+        at = 512 + (offset if st[key].element_size() == 4 else offset // 4 * 3)
+        mid = raw[at: at + st[key].numel() * st[key].element_size()]
         mid.copy_(st[key].view(torch.uint8).reshape(-1))
         st[key] = mid.view(st[key].dtype).view(st[key].shape)
-        around.append((raw, mid.numel()))
+        around.append((raw, at, mid.numel()))
     opt.prime_for_cuda_graph()
-    opt.step()
-    torch.cuda.synchronize()
+    _check_step(opt, opt.step)
     assert (buf[:32] == 5.0).all() and (buf[32 + n:] == 5.0).all()
     assert all(v.float().ne(0).all() for key, v in st.items() if key in ("exp_avg", "exp_avg_sq", "exp_avg_q", "exp_avg_sq_q"))
-    for raw, k in around:
-        assert (raw[:512] == 77).all() and (raw[512 + k:] == 77).all()
+    for raw, at, k in around:
+        assert (raw[:at] == 77).all() and (raw[at + k:] == 77).all()
 
 
 @pytest.mark.parametrize("kind", ["fp32", "8bit"])
@@ -317,6 +343,9 @@ def test_a_gradient_that_is_not_finite_stays_with_its_element(kind):
     same[300] = same[1000] = False
     assert not torch.isfinite(ps[0].data[[300, 1000]]).any()
     assert torch.isfinite(ps[0].data[same]).all()
+    if kind == "8bit":      # moments that are no numbers are held as some
+        st = a.state[ps[0]]
+        assert all(torch.isfinite(st[key].float()).all() for key in ("exp_avg_q", "exp_avg_sq_q"))
     if kind == "8bit":
         same[768:1024] = False
     assert torch.equal(ps[0].data[same], qs[0].data[same])
