@@ -537,3 +537,121 @@ def test_training_with_all_of_them():
         _check_step(o32, o32.step)
         want = math.sqrt(sum((p.grad.double() ** 2).sum().item() for p in b.parameters()))
         _check_step(o, o.step, min(1.0, 0.1 / (want + 1e-6)), 6 * EPS24)
+
+
+def test_came_and_adamw_tensors_share_a_plan():
+    """One tensor table with both kinds steps each as a table of its own would."""
+    import came_b200
+    from came_b200.engine import DevicePlan
+
+    def make():
+        ps = _params([(96, 130), (300,), (64, 256), (513,), (33, 70)], torch.bfloat16)
+        _set_grads(ps, 5)
+        return ps, came_b200.CAMECUDA(ps[:2], lr=1e-3, weight_decay=0.1), came_b200.AdamW8bit(ps[2:4], **HYPER, max_grad_norm=0.1), came_b200.AdamW(
+            ps[4:], **HYPER, max_grad_norm=0.1)
+
+    (pa, ca, a8, _), (pb, cb, b8, _) = make(), make()
+    opts, entries, hypers = (ca, a8), [], []
+    for o in opts:
+        es, hs, _ = o._collect()
+        for e in es:
+            e.group += len(hypers)
+        entries += es
+        hypers += hs
+    plan = DevicePlan(torch.device("cuda", 0), entries)
+    for k in range(3):
+        plan.step(hypers)
+        cb.step(), b8.step()
+        for p, q in zip(pa[:4], pb[:4]):
+            assert torch.equal(p.data, q.data)
+        assert plan.grad_norm.item() == b8.grad_norm.item()
+    assert a8.state[pa[2]]["step"].item() == 3
+    plan.close()
+
+
+def test_nothing_of_adamw_is_pushed():
+    """The push mode of the weight exchange does not know these tensors: they are reported as to be copied, and are not stored."""
+    import came_b200
+    flat = torch.zeros(8192, device="cuda", dtype=torch.bfloat16)
+    p = torch.nn.Parameter(flat[:4096].view(64, 64))
+    p.grad = torch.ones_like(p)
+    opt = came_b200.AdamW([p], **HYPER)
+    opt.prime_for_cuda_graph()
+    mirror = torch.zeros_like(flat)
+    opt._engine.set_push(flat.data_ptr(), flat.numel() * 2, [mirror.data_ptr()])
+    (plan,) = opt._engine.plans.values()
+    opt.step()
+    torch.cuda.synchronize()
+    assert plan.pushed() == [False] and not mirror.any() and flat[:4096].all()
+
+
+def test_two_optimizers_on_two_streams():
+    """Launches that overlap at their ends, of optimizers that have nothing to do with one another."""
+    import came_b200
+    sets = [_params([(500, 512), (129,), (2000, 33)], torch.bfloat16, s) for s in (1, 2, 1, 2)]
+    for i, ps in enumerate(sets):
+        _set_grads(ps, 10 + i % 2)
+    opts = [came_b200.AdamW8bit(ps, **HYPER, max_grad_norm=0.5) for ps in sets]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    norms = []
+    for _ in range(20):
+        for s, o, ps in zip(streams, opts[:2], sets[:2]):
+            with torch.cuda.stream(s):
+                o.step()
+                norms.append(came_b200.clip_grad_norm_(ps, math.inf))
+    torch.cuda.synchronize()
+    for o in opts[2:]:
+        for _ in range(20):
+            o.step()
+    torch.cuda.synchronize()
+    for a, b in zip(sets[:2], sets[2:]):
+        assert all(torch.equal(p.data, q.data) for p, q in zip(a, b))
+    assert len({n.item() for n in norms[::2]}) == len({n.item() for n in norms[1::2]}) == 1
+
+
+@pytest.mark.parametrize("kind", ["fp32", "8bit"])
+def test_refusals(kind):
+    p = torch.nn.Parameter(torch.zeros(8, 8, device="cuda", dtype=torch.float64))
+    p.grad = torch.ones_like(p)
+    with pytest.raises(RuntimeError, match="float64"):
+        _cls(kind)([p]).step()
+    ps = _params([(8, 8), (5,)], torch.float32)
+    _set_grads(ps, 0)
+    opt = _cls(kind)([{"params": [torch.nn.Parameter(torch.zeros(1, device="cuda"))]} for _ in range(64)] + [{"params": ps}], lr=1e-3)
+    with pytest.raises(RuntimeError, match="param_groups"):
+        opt.step()
+    opt = _cls(kind)(ps, lr=1e-3)
+    opt.step()
+    opt.param_groups[0]["betas"] = (0.9, 1.0)
+    before = [q.detach().clone() for q in ps]
+    with pytest.raises(ValueError, match="betas"):
+        opt.step()
+    assert all(torch.equal(a, b.data) for a, b in zip(before, ps))
+    opt.param_groups[0]["betas"] = (0.9, 0.99)
+    st = opt.state[ps[0]]
+    key = "exp_avg" if kind == "fp32" else "exp_avg_q"
+    st[key] = torch.zeros(3, device="cuda", dtype=st[key].dtype)
+    with pytest.raises(RuntimeError, match="shape"):
+        opt.prime_for_cuda_graph()
+    s = torch.nn.Parameter(torch.zeros(4, 4, device="cuda"))
+    s.grad = torch.sparse_coo_tensor(torch.tensor([[0], [0]]), torch.tensor([1.0]), (4, 4)).cuda()
+    with pytest.raises(RuntimeError, match="sparse"):
+        _cls(kind)([s]).step()
+
+
+def test_eager_steps_between_replays():
+    import came_b200
+    pe, pg = _params([(300, 40), (77,)], torch.float32), _params([(300, 40), (77,)], torch.float32)
+    oe, og = came_b200.AdamW8bit(pe, **HYPER), came_b200.AdamW8bit(pg, **HYPER)
+    _set_grads(pe, 3), _set_grads(pg, 3)
+    og.prime_for_cuda_graph()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        og.step()
+    for k in range(6):
+        oe.step()
+        graph.replay() if k % 3 else og.step()
+    torch.cuda.synchronize()
+    assert all(torch.equal(p.data, q.data) for p, q in zip(pe, pg)) and og.state[pg[0]]["step"].item() == 6
