@@ -447,8 +447,14 @@ PyObject* clip_grad_norm(PyObject*, PyObject* args) {
     std::vector<CameGradRef> refs;
     at::Tensor first;
     refs.reserve((size_t)PyList_GET_SIZE(list));
+    PyTypeObject* known = nullptr;      // asking whether a parameter is a tensor takes as long as the rest: once per type
     for (Py_ssize_t i = 0; i < PyList_GET_SIZE(list); ++i) {
-        const at::Tensor& t = tensor_of(PyList_GET_ITEM(list, i));
+        PyObject* const o = PyList_GET_ITEM(list, i);
+        if (Py_TYPE(o) != known) {
+            tensor_of(o);
+            known = Py_TYPE(o);
+        }
+        const at::Tensor& t = THPVariable_Unpack(o);
         const at::Tensor& g = of_params ? t.grad() : t;
         if (!g.defined()) continue;
         if (g.layout() != at::kStrided || !g.is_cuda() || (first.defined() && g.device() != first.device())) Py_RETURN_NONE;

@@ -743,6 +743,8 @@ class AdamW(_CameB200Optimizer):
         entries, hypers, copy_backs = super()._collect()
         if self._max_grad_norm is not None and len({e.p.device for e in entries}) > 1:
             raise RuntimeError("max_grad_norm needs all parameters on one device")
+        if len({e.p.data_ptr() for e in entries}) != len(entries):
+            raise ValueError("a parameter is listed twice: its two steps would race")
         return entries, hypers, copy_backs
 
     def load_state_dict(self, state_dict):

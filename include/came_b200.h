@@ -178,7 +178,7 @@ int came_b200_step(came_plan_t* plan, const CameHyper* hypers, int n_groups, cam
  * than 2^-16 unless the whole block is zero, is rounded to the format after a number r has been added to its fp32 bits and
  * the low 20 (m) / 21 (v) bits have been cleared: with h = mix((e >> 3) + mix(t)) * (0x9E3779B1 * (2 (e & 7) + 1)) mod 2^32,
  * e the flat index of the element and mix the 32-bit mixer x ^= x >> 16, x *= 0x7feb352d, x ^= x >> 15, x *= 0x846ca68b,
- * x ^= x >> 16: r = h mod 2^20 (m), h >> 11 (v).  A moment that is no number is held as one.
+ * x ^= x >> 16: r = h mod 2^20 (m), h >> 11 (v).  A moment that is NaN is held as some finite value.
  * The norm N of the last step lies in the workspace, at the byte offset that came_b200_plan_norm_offset gives (one fp32
  * number; -1 when the plan takes none).
  */

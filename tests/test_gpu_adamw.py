@@ -2,6 +2,7 @@
 step must leave alone; captured, moved, sharded and resumed steps."""
 import copy
 import math
+import warnings
 
 import pytest
 import torch
@@ -585,6 +586,18 @@ def test_nothing_of_adamw_is_pushed():
     assert plan.pushed() == [False] and not mirror.any() and flat[:4096].all()
 
 
+@pytest.mark.parametrize("kind", ["fp32", "8bit"])
+def test_the_kernels_that_run(kind):
+    from tests.parity_util import kernels_of
+    ps = _params([(300, 40), (77,)], torch.bfloat16)
+    _set_grads(ps, 1)
+    name = {"fp32": "adamw", "8bit": "adamw8"}[kind]
+    for limit, names in ((None, {name}), (1.0, {name, "grad_norm"})):
+        opt = _cls(kind)(ps, **HYPER, max_grad_norm=limit)
+        opt.step()
+        assert kernels_of(opt) == names and opt.last_step_launches == len(names)
+
+
 def test_two_optimizers_on_two_streams():
     """Launches that overlap at their ends, of optimizers that have nothing to do with one another."""
     import came_b200
@@ -634,6 +647,13 @@ def test_refusals(kind):
     st[key] = torch.zeros(3, device="cuda", dtype=st[key].dtype)
     with pytest.raises(RuntimeError, match="shape"):
         opt.prime_for_cuda_graph()
+    with pytest.raises(ValueError, match="twice"), warnings.catch_warnings():
+        warnings.simplefilter("ignore")
+        _cls(kind)([ps[1], ps[1]]).step()
+    with pytest.raises(ValueError, match="twice"):
+        alias = torch.nn.Parameter(ps[1].data)
+        alias.grad = ps[1].grad
+        _cls(kind)([ps[1], alias]).step()
     s = torch.nn.Parameter(torch.zeros(4, 4, device="cuda"))
     s.grad = torch.sparse_coo_tensor(torch.tensor([[0], [0]]), torch.tensor([1.0]), (4, 4)).cuda()
     with pytest.raises(RuntimeError, match="sparse"):
