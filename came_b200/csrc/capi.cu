@@ -63,7 +63,7 @@ inline int elem_bytes(int dt) { return dt == CAME_DT_F32 ? 4 : 2; }
 inline bool is_adamw(const CameTensorDesc& d) { return d.mode == CAME_MODE_ADAMW || d.mode == CAME_MODE_ADAMW8; }
 inline bool is_nd(const CameTensorDesc& d) { return d.cols != 0 && d.batch > 1 && !is_adamw(d); }
 inline int64_t elements(const CameTensorDesc& d) { return d.rows * (d.cols ? d.cols : 1) * (d.batch > 1 ? (int64_t)d.batch : 1); }
-// (AdamW kernels copy from the 16-byte boundaries around an element)
+// (AdamW kernels take an element wherever it is aligned as one)
 inline bool on_elements(const CameTensorDesc& d) {
     auto on = [](const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % (uintptr_t)bytes == 0; };
     const int state = d.mode == CAME_MODE_ADAMW ? 4 : 1;
