@@ -73,13 +73,8 @@ __device__ __forceinline__ uint32_t mix32(uint32_t x) {
 template <int TOP>
 __device__ __forceinline__ uint32_t e8m0_scale(uint32_t top_bits) { return (uint32_t)max((int)(top_bits >> 23) - TOP, 1); }
 __device__ __forceinline__ float e8m0_value(uint32_t byte) { return __uint_as_float(byte ? byte << 23 : 0x00400000u); }      // (byte 0 is 2^-127)
-__device__ __forceinline__ float e8m0_inverse(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }      // (byte in [1, 248])
 
-// stochastic rounding: r < 2^BITS is added to the mantissa below the bits that stay, the rest is cut off
-template <int BITS>
-__device__ __forceinline__ float dither(float y, uint32_t r) { return __uint_as_float((__float_as_uint(y) + r) & ~((1u << BITS) - 1u)); }
-
-// two codes of a word of four (the lower or the upper two) <-> fp32
+// two codes of a word of four (the lower or the upper two) to fp32
 __device__ __forceinline__ float2 e4m3_pair(uint32_t w, int upper) {
     uint32_t h;
     const uint16_t two = (uint16_t)(upper ? w >> 16 : w);
@@ -89,16 +84,6 @@ __device__ __forceinline__ float2 e4m3_pair(uint32_t w, int upper) {
 __device__ __forceinline__ float2 e5m2_pair(uint32_t w, int upper) {      // (e5m2 is the upper byte of fp16)
     const uint32_t h = __byte_perm(w, 0u, upper ? 0x3424u : 0x1404u);
     return __half22float2(*reinterpret_cast<const __half2*>(&h));
-}
-__device__ __forceinline__ uint32_t e4m3_codes(float lo, float hi) {
-    uint16_t c;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(c) : "f"(hi), "f"(lo));
-    return c;
-}
-__device__ __forceinline__ uint32_t e5m2_codes(float lo, float hi) {
-    uint16_t c;
-    asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(c) : "f"(hi), "f"(lo));
-    return c;
 }
 
 // ------------------------------------------------------------------------------------------

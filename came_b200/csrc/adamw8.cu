@@ -3,8 +3,8 @@
 // m is held as e4m3, v as e5m2 (its root then has the range and the relative step of m), both times a scale 2^k (one e8m0
 // byte per 256 elements) that puts the exponent of the block's largest magnitude at 2^7 resp. 2^14.  A scale that is a power
 // of two leaves the grid where it is from step to step, so that only what a moment gained is rounded, and it is rounded
-// stochastically: a uniform number is added below the last mantissa bit that is kept, the rest is cut off.  Rounded to
-// nearest, v would never fall at b2 = 0.999 (a step moves it by 0.1 %, half a spacing is 7 to 12 %).
+// stochastically on the format's whole grid, subnormals included.  Rounded to nearest, v would never fall at b2 = 0.999 (a step
+// moves it by 0.1 %, half a spacing is 7 to 12 %), and an m of few subnormal units would never die out at b1 = 0.9.
 // The random bits are a hash of the element's index and t: no state, the same in every run.
 //
 // A warp owns blocks of 256 elements, a lane 8 consecutive elements of each; the block's largest magnitudes are one warp
@@ -13,9 +13,11 @@
 // from the boundaries around them and shifted as they are read.
 //
 // Bound by instructions first, by DRAM close behind (10.03 bytes an element in 16-bit types): one element per lane and step takes
-// 54 instructions; packed arithmetic, whole blocks without questions per block (span8_fast) and the scale of v in the same
-// addition as its random bits leave 33.  256 M bf16 elements: 406 us (97 % of the copy rate); under the power cap, back to
+// 54 instructions; packed arithmetic, whole blocks without questions per block (span8_fast) and codes that are cut out of the
+// rounded bits instead of converted leave 33.  256 M bf16 elements: 405 us (97 % of the copy rate); under the power cap, back to
 // back, the clock falls to 1.6-1.8 GHz and 1.26 G elements take 2.06-2.2 ms (88-94 %).
+#include <cfloat>
+
 #include "adamw.cuh"
 #include "launch.h"
 #include "pipeline.cuh"
@@ -124,6 +126,25 @@ struct Result8 {
     uint32_t m_top, v_top;      // bits of the block's largest magnitudes
 };
 
+// Stochastic rounding on the grid of an 8-bit format with SHIFT = 23 - (its mantissa bits): floor(|y| / u + r / 2^SHIFT) u, u the
+// spacing at y.  y = x / 2^k is brought down by as much as lies between the least normal numbers of fp32 and of the format, 2^-120
+// for e4m3 and 2^-112 for e5m2.  The spacing then is bit SHIFT of the fp32 number whatever its size, subnormals included:
+// r < 2^SHIFT is added to the bits, and the code stands above bit SHIFT.  The product is truncated, which loses nothing
+// of the floor.  Two neighbours become the upper and the lower half of a word, and from there bytes.
+__device__ __forceinline__ uint32_t e4m3_halves(u64 x, uint32_t r0, uint32_t r1) {      // codes in the upper bytes
+    const uint32_t w = __byte_perm(__float_as_uint(x.x) + (r0 & 0xfffffu), __float_as_uint(x.y) + (r1 & 0xfffffu), 0x7632u);
+    return ((w << 4) & 0x7fff7fffu) | (w & 0x80008000u);
+}
+__device__ __forceinline__ uint32_t e5m2_halves(u64 x, uint32_t r0, uint32_t r1, int least) {      // (no sign)
+    const int w0 = max((int)(__float_as_uint(x.x) + (r0 >> 11)), least), w1 = max((int)(__float_as_uint(x.y) + (r1 >> 11)), least);
+    return __byte_perm((uint32_t)w0, (uint32_t)w1, 0x7632u) << 3;
+}
+// 2^-k 2^-120 resp. 2^-k 2^-112 for a scale byte k + 127; above these bytes the factor would leave fp32: part of it is taken
+// off before
+constexpr uint32_t M_BYTE_HIGH = 134, V_BYTE_HIGH = 142, M_PART = 115, V_PART = 100;
+__device__ __forceinline__ float m_factor(uint32_t byte) { return __uint_as_float((M_BYTE_HIGH - byte) << 23); }
+__device__ __forceinline__ float v_factor(uint32_t byte) { return __uint_as_float((V_BYTE_HIGH - byte) << 23); }
+
 // Elements go in pairs through the packed fp32 instructions.  Moments: every product and sum is rounded by itself, as separate
 // tensor operations round them, so that codes can be compared bit for bit (the scale is a power of two: scale * beta * code is
 // beta * value).  m_keep, v_keep: beta * scale; group: index of the 8 elements in their tensor.
@@ -150,38 +171,30 @@ __device__ __forceinline__ void block8_math(Result8& out, const uint32_t* pw, co
     }
     out.m_top = __reduce_max_sync(0xffffffffu, __float_as_uint(m_big));
     out.v_top = __reduce_max_sync(0xffffffffu, __float_as_uint(v_big));
-    const u64 m_inv = splat(e8m0_inverse(e8m0_scale<7>(out.m_top)));
+    uint32_t m_byte = e8m0_scale<7>(out.m_top), v_byte = e8m0_scale<14>(out.v_top);
+    if (m_byte >= M_BYTE_HIGH || v_byte >= V_BYTE_HIGH) {      // |m| from 2^14, v from 2^29 on
+        const float m_part = m_byte >= M_BYTE_HIGH ? 0x1p-115f : 1.0f, v_part = v_byte >= V_BYTE_HIGH ? 0x1p-100f : 1.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            m[j] = __fmul2_rz(m[j], splat(m_part));      // (truncated twice is truncated once)
+            v[j] = __fmul2_rz(pk(fminf(v[j].x, FLT_MAX), fminf(v[j].y, FLT_MAX)), splat(v_part));
+        }
+        if (m_byte >= M_BYTE_HIGH) m_byte -= M_PART;
+        if (v_byte >= V_BYTE_HIGH) v_byte -= V_PART;
+    }
+    const u64 m_down = splat(m_factor(m_byte)), v_down = splat(v_factor(v_byte));
+    const int least = out.v_top ? 1 << 21 : 0;      // v stays above zero (its root divides): at least 2^-16 after scaling; a block of zeros stays zero
     const uint32_t h = mix32(group + k.key);
-    uint32_t r[8], mc[4], vc[4];
+    uint32_t r[8], mh[4], vh[4];
 #pragma unroll
     for (int i = 0; i < 8; ++i) r[i] = h * (0x9E3779B1u * (2u * i + 1u));
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const u64 x = mul2(m[j], m_inv);
-        mc[j] = e4m3_codes(dither<20>(x.x, r[2 * j] & 0xfffffu), dither<20>(x.y, r[2 * j + 1] & 0xfffffu));
+        mh[j] = e4m3_halves(__fmul2_rz(m[j], m_down), r[2 * j], r[2 * j + 1]);
+        vh[j] = e5m2_halves(__fmul2_rz(v[j], v_down), r[2 * j], r[2 * j + 1], least);
     }
-    // v stays above zero (its root divides): at least 2^-16 after scaling; a block of zeros stays zero
-    if (out.v_top >= 32u << 23) {
-        // The scale goes into the exponent with the random bits; what is less than 2^-16 then, or below zero (a v without an
-        // exponent of its own among them: its block's is 32 at least), is 2^-16 in one instruction.
-        const uint32_t shift = (141u << 23) - (out.v_top & 0x7f800000u);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int y0 = __viaddmax_s32(__float_as_int(v[j].x), (int)((r[2 * j] >> 11) + shift), 111 << 23);
-            const int y1 = __viaddmax_s32(__float_as_int(v[j].y), (int)((r[2 * j + 1] >> 11) + shift), 111 << 23);
-            vc[j] = e5m2_codes(__int_as_float(y0 & ~0x1fffff), __int_as_float(y1 & ~0x1fffff));
-        }
-    } else {
-        const u64 v_inv = splat(e8m0_inverse(e8m0_scale<14>(out.v_top)));
-        const float least = out.v_top ? 0x1p-16f : 0.0f;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const u64 y = mul2(v[j], v_inv);
-            vc[j] = e5m2_codes(dither<21>(fmaxf(y.x, least), r[2 * j] >> 11), dither<21>(fmaxf(y.y, least), r[2 * j + 1] >> 11));
-        }
-    }
-    out.m = make_uint2(__byte_perm(mc[0], mc[1], 0x5410u), __byte_perm(mc[2], mc[3], 0x5410u));
-    out.v = make_uint2(__byte_perm(vc[0], vc[1], 0x5410u), __byte_perm(vc[2], vc[3], 0x5410u));
+    out.m = make_uint2(__byte_perm(mh[0], mh[1], 0x7531u), __byte_perm(mh[2], mh[3], 0x7531u));
+    out.v = make_uint2(__byte_perm(vh[0], vh[1], 0x7531u), __byte_perm(vh[2], vh[3], 0x7531u));
 }
 
 // Scales of a warp's blocks: lane l holds those of block l

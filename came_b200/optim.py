@@ -770,8 +770,9 @@ class AdamW8bit(AdamW):
     """AdamW with two bytes of state per element.  Per block of 256 flat elements the first moment is held as float8 e4m3
     codes (`exp_avg_q`), the second as e5m2 codes (`exp_avg_sq_q`), each with a power-of-two scale in one e8m0 byte
     (`exp_avg_scale`, `exp_avg_sq_scale`): the value is `code.float() * scale.float()`.  Both are rounded stochastically, with
-    bits hashed from the element's index and the step count: two runs give the same bits.  Rounded to nearest, the second
-    moment could not follow at betas[1] = 0.999, where a step moves it by less than half a spacing.  The update itself uses
+    bits hashed from the element's index and the step count, over the whole range of the formats: two runs give the same bits.
+    Rounded to nearest, the second moment could not follow at betas[1] = 0.999, where a step moves it by less than half a
+    spacing, and the first could not die out.  The update itself uses
     the moments before they are rounded."""
 
     _layout = "adamw8"

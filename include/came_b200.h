@@ -174,11 +174,12 @@ int came_b200_step(came_plan_t* plan, const CameHyper* hypers, int n_groups, cam
  *     m' = beta1 m + (1 - beta1) c g          v' = beta2 v + (1 - beta2) (c g)^2
  *     p' = p (1 - lr wd) - lr / (1 - beta1^t) * m' / (sqrt(v') / sqrt(1 - beta2^t) + eps)
  * p' uses m' and v' before they are rounded to float8.  CAME_MODE_ADAMW8 holds a block of 256 flat elements as code * 2^k:
- * 2^k puts the exponent of the largest magnitude at 2^7 (m) resp. 2^14 (v), at least k = -126; y = x / 2^k, for v no less
- * than 2^-16 unless the whole block is zero, is rounded to the format after a number r has been added to its fp32 bits and
- * the low 20 (m) / 21 (v) bits have been cleared: with h = mix((e >> 3) + mix(t)) * (0x9E3779B1 * (2 (e & 7) + 1)) mod 2^32,
- * e the flat index of the element and mix the 32-bit mixer x ^= x >> 16, x *= 0x7feb352d, x ^= x >> 15, x *= 0x846ca68b,
- * x ^= x >> 16: r = h mod 2^20 (m), h >> 11 (v).  A moment that is NaN is held as some finite value.
+ * 2^k puts the exponent of the largest magnitude at 2^7 (m) resp. 2^14 (v), at least k = -126.  y = x / 2^k, for v no less
+ * than 2^-16 unless the whole block is zero, is held as sign(y) * floor(|y| / u + r) * u, u the format's spacing at y (below the
+ * least normal number that of the subnormals, 2^-9 resp. 2^-16): 0 <= r < 1 is r = (s mod 2^20) / 2^20 (m), (s >> 11) / 2^21
+ * (v), with s = mix((e >> 3) + mix(t)) * (0x9E3779B1 * (2 (e & 7) + 1)) mod 2^32, e the flat index of the element and mix the
+ * 32-bit mixer x ^= x >> 16, x *= 0x7feb352d, x ^= x >> 15, x *= 0x846ca68b, x ^= x >> 16.  A moment that is NaN is held as some
+ * value, one that is infinite as the block's largest code or next to it.
  * The norm N of the last step lies in the workspace, at the byte offset that came_b200_plan_norm_offset gives (one fp32
  * number; -1 when the plan takes none).
  */

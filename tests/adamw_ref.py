@@ -47,22 +47,23 @@ def blocks(x, fill=0.0):
 
 
 def encode(x, which, t):
-    """(values the codes stand for before the scale, scales as fp32) of an fp32 tensor, blockwise, at step count t; every
-    operation is exact, so that a kernel that has the same fp32 x has the same codes."""
+    """(values the codes stand for before the scale, scales as fp32) of an fp32 tensor, blockwise, at step count t: y = x / scale
+    becomes sign(y) floor(|y| / u + r / 2^drop) u, u the format's spacing at y, that of its subnormals below the least normal
+    number.  In 64 bits from the definition; every operation is exact."""
     top, drop, least, _, _, dtype = FORMATS[which]
     n = x.numel()
     h = random_bits(n, t, x.device)
     r = (h & 0xFFFFF) if which == "m" else h >> 11
-    b = blocks(x)
+    b = blocks(x).double()
     a = b.abs().amax(1, keepdim=True)
     e = (torch.frexp(a)[1] - 1 - top).clamp(-126, 127)
     scale = torch.where(a > 0, torch.ldexp(torch.ones_like(a), e), torch.full_like(a, 2.0 ** -126))
     y = b / scale
     if least is not None:
         y = torch.where(a > 0, y.clamp(min=least), y)
-    bits = (y.view(torch.int32) + blocks(r).to(torch.int32)) & ~((1 << drop) - 1)
-    codes = bits.view(torch.float32).to(dtype)
-    return codes.reshape(-1)[:n].view(x.shape), scale[:, 0]
+    u = spacing(y, which)
+    q = torch.floor(y.abs() / u + blocks(r).double() / 2.0 ** drop) * u * torch.sign(y)
+    return q.to(dtype).reshape(-1)[:n].view(x.shape), scale[:, 0].float()
 
 
 def decode(codes, scale):
