@@ -62,10 +62,10 @@ struct LaunchItem {
 inline int elem_bytes(int dt) { return dt == CAME_DT_F32 ? 4 : 2; }
 inline bool is_adamw(const CameTensorDesc& d) { return d.mode == CAME_MODE_ADAMW || d.mode == CAME_MODE_ADAMW8; }
 inline bool is_nd(const CameTensorDesc& d) { return d.cols != 0 && d.batch > 1 && !is_adamw(d); }
+inline bool on(const void* p, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 inline int64_t elements(const CameTensorDesc& d) { return d.rows * (d.cols ? d.cols : 1) * (d.batch > 1 ? (int64_t)d.batch : 1); }
 // (AdamW kernels take an element wherever it is aligned as one)
 inline bool on_elements(const CameTensorDesc& d) {
-    auto on = [](const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % (uintptr_t)bytes == 0; };
     const int state = d.mode == CAME_MODE_ADAMW ? 4 : 1;
     return on(d.p, elem_bytes(d.p_dtype)) && on(d.g, elem_bytes(d.g_dtype)) && on(d.m, state) && on(d.sq_row, state) && on(d.res_row, 4);
 }
@@ -82,7 +82,6 @@ struct VecFlags {
 VecFlags vec_flags(const CameTensorDesc& d, bool fast) {
     VecFlags f{0, 0, 0};
     if (is_adamw(d)) {      // eight elements of a tensor by one access
-        auto on = [](const void* p, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; };
         if (d.mode == CAME_MODE_ADAMW8) f.v = on(d.m, 8) && on(d.sq_row, 8) ? 8 : 1;      // (parameters and gradients may start anywhere)
         else f.v = on(d.p, 8 * elem_bytes(d.p_dtype)) && on(d.g, 8 * elem_bytes(d.g_dtype)) && on(d.m, 32) && on(d.sq_row, 32) ? 8 : 1;
         return f;
@@ -965,10 +964,12 @@ size_t came_b200_clip_workspace_bytes(int n_tensors) { return n_tensors < 0 ? 0 
 int came_b200_clip_grad_norm(const CameGradRef* grads, int n_tensors, float max_norm, float* norm, void* workspace,
                              size_t workspace_bytes, came_stream_t stream) {
     if (n_tensors < 0 || (n_tensors > 0 && !grads) || !norm) return fail(CAME_E_INVALID, "clip_grad_norm: null argument or negative count");
+    if (!on(norm, sizeof(float))) return fail(CAME_E_INVALID, "clip_grad_norm: norm is not 4-byte aligned");
     if (!(max_norm >= 0.0f)) return fail(CAME_E_INVALID, "clip_grad_norm: max_norm must be >= 0");
     for (int i = 0; i < n_tensors; ++i) {
         if (grads[i].n < 0 || (grads[i].n > 0 && !grads[i].g)) return fail(CAME_E_INVALID, "clip_grad_norm: tensor %d: null pointer or negative size", i);
         if (grads[i].dtype < CAME_DT_F32 || grads[i].dtype > CAME_DT_BF16) return fail(CAME_E_INVALID, "clip_grad_norm: tensor %d: bad dtype", i);
+        if (grads[i].n > 0 && !on(grads[i].g, elem_bytes(grads[i].dtype))) return fail(CAME_E_INVALID, "clip_grad_norm: tensor %d: not aligned to its elements", i);
         if (grads[i].n > 4000000000000LL) return fail(CAME_E_UNSUPPORTED, "clip_grad_norm: tensor %d: too many elements", i);
     }
     if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 8 != 0 || workspace_bytes < came_b200_clip_workspace_bytes(n_tensors))

@@ -189,7 +189,8 @@ int64_t came_b200_plan_norm_offset(const came_plan_t* plan);
  * Norm of the gradients of many tensors, and clip by it (no counterpart in the reference): *norm (device memory) becomes
  * N = sqrt(sum of all squares), then every gradient is multiplied by min(1, max_norm / (N + 1e-6)) in place (left alone where
  * that is 1; with a N that is not a number all become NaN).  max_norm >= 0; infinity asks for the norm alone.  `grads`: host
- * memory, read before the call returns; dense tensors of n elements each, in any order of dimensions, that do not overlap.
+ * memory, read before the call returns; dense tensors of n elements each, in any order of dimensions, that do not overlap,
+ * aligned to their elements (others are refused).
  * workspace: came_b200_clip_workspace_bytes(n_tensors) bytes of device memory, 8-byte aligned, used until the call's kernels
  * are done.  May be captured into a CUDA graph (addresses and max_norm are those of the capture).
  */
