@@ -81,6 +81,7 @@ SYMBOLS = {
     "came_b200_clip_workspace_bytes": (C.c_size_t, [C.c_int]),
     "came_b200_clip_grad_norm": (C.c_int, [C.POINTER(CameGradRef), C.c_int, C.c_float, C.c_void_p, C.c_void_p, C.c_size_t,
                                            C.c_void_p]),
+    "came_b200_plan_captured": (C.c_int, [C.c_void_p]),
     "came_b200_plan_set_hyper": (C.c_int, [C.c_void_p, C.POINTER(CameHyper), C.c_int]),
     "came_b200_peer_copy_async": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_int, C.c_void_p]),
     "came_b200_ipc_export": (C.c_int, [C.c_void_p, C.c_char_p, C.POINTER(C.c_uint64)]),

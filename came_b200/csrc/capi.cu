@@ -416,6 +416,7 @@ struct came_plan {
     // CUDA graph (the graph's copy node reads it again at every replay)
     CameHyper* graph_hyp = nullptr;
     int graph_groups = 0;
+    int captured_groups = 0;       // records of a step that was captured: from then on the addresses stay
     ~came_plan() {
         for (auto& t : timed) { cudaEventDestroy(t.t0); cudaEventDestroy(t.t1); }
         if (graph_hyp) cudaFreeHost(graph_hyp);
@@ -840,6 +841,10 @@ int came_b200_plan_set_pointers(came_plan_t* plan, const void* const* g, void* c
     if (!plan) return fail(CAME_E_INVALID, "set_pointers: plan is null");
     if (n_tensors != plan->n_tensors) return fail(CAME_E_INVALID, "set_pointers: %d tensors given, plan has %d", n_tensors, plan->n_tensors);
     if (!g && !p) return CAME_OK;
+    if (plan->captured_groups)
+        for (int i = 0; i < n_tensors; ++i)
+            if ((g && g[i] != plan->descs[i].g) || (p && p[i] != plan->descs[i].p))
+                return fail(CAME_E_INVALID, "set_pointers: tensor %d moves, but a captured step reads this plan's addresses; create a new plan", i);
     // (only the addresses change: nothing is copied back when one of them is refused)
     const bool fast = !disable_fast();
     for (int i = 0; i < n_tensors; ++i) {
@@ -876,6 +881,8 @@ int came_b200_plan_set_hyper(came_plan_t* plan, const CameHyper* hypers, int n_g
     return stage_graph_hypers("plan_set_hyper", plan, hypers, n_groups);
 }
 
+int came_b200_plan_captured(const came_plan_t* plan) { return plan ? plan->captured_groups : 0; }
+
 int came_b200_step(came_plan_t* plan, const CameHyper* hypers, int n_groups, came_stream_t stream) {
     int rc = check_hypers("step", plan, hypers, n_groups);
     if (rc != CAME_OK) return rc;
@@ -893,6 +900,7 @@ int came_b200_step(came_plan_t* plan, const CameHyper* hypers, int n_groups, cam
         rc = stage_graph_hypers("step", plan, hypers, n_groups);
         if (rc != CAME_OK) return rc;
         src = plan->graph_hyp;
+        plan->captured_groups = n_groups;
     }
     // The whole-step kernel takes a few records as kernel arguments; a captured step reads them from memory, so that a
     // replay sees new values.

@@ -123,9 +123,9 @@ class DevicePlan:
         self.n = len(entries)
         self.structure = tuple(e.structure_key() for e in entries)
         self.addresses = tuple((e.p.data_ptr(), e.g.data_ptr()) for e in entries)
-        # AdamW: the plan keeps the states it points at
-        self.keep = [(e.m, e.m_absmax, e.sq_row, e.sq_row_absmax, e.res_row) for e in entries
-                     if e.mode in (_lib.MODE_ADAMW, _lib.MODE_ADAMW8)]
+        # the plan keeps the states it points at
+        self.keep = [(e.m, e.m_absmax, e.sq_row, e.sq_row_absmax, e.sq_col, e.sq_col_absmax, e.res_row, e.res_row_absmax, e.res_col,
+                      e.res_col_absmax) for e in entries]
         descs = (CameTensorDesc * self.n)()
         for d, e in zip(descs, entries):
             elementwise = e.mode in (_lib.MODE_ADAMW, _lib.MODE_ADAMW8)
@@ -202,6 +202,11 @@ class DevicePlan:
         return None if at < 0 else self.workspace[at:at + 4].view(torch.float32).reshape(())
 
     @property
+    def captured(self) -> int:
+        """Number of records that a captured step of this plan reads; 0: none was captured."""
+        return self.lib.came_b200_plan_captured(self.handle)
+
+    @property
     def last_launches(self) -> int:
         return self.lib.came_b200_plan_last_launches(self.handle)
 
@@ -238,10 +243,12 @@ class DevicePlan:
 
 class StepEngine:
     """Keeps one DevicePlan per device alive across steps and rebuilds it only when the set of
-    tensors, their state buffers or their alignment class changes."""
+    tensors, their state buffers or their alignment class changes.  A plan whose step has been captured is read at every
+    replay: it is never closed nor re-pointed, another takes its place in eager steps."""
 
     def __init__(self):
         self.plans: dict = {}
+        self.retired: list = []      # captured plans that eager steps no longer use, oldest first
         self.push = None      # (local_base, local_bytes, [peer bases]) applied to every plan that is (re)built
 
     def set_push(self, local_base: int, local_bytes: int, peer_bases: list) -> None:
@@ -250,10 +257,15 @@ class StepEngine:
         for plan in self.plans.values():
             plan.set_push(*self.push)
 
-    def invalidate(self) -> None:
-        for plan in self.plans.values():
+    def _drop(self, plan) -> None:
+        if plan.captured:
+            self.retired.append(plan)
+        else:
             plan.close()
-        self.plans.clear()
+
+    def invalidate(self) -> None:
+        while self.plans:
+            self._drop(self.plans.popitem()[1])
 
     def prepare(self, entries: list) -> list:
         by_dev: dict = {}
@@ -264,20 +276,30 @@ class StepEngine:
             plan = self.plans.get(dev)
             structure = tuple(e.structure_key() for e in es)
             if plan is None or plan.structure != structure or not plan.repoint(es):
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("the tensors of this step are not those that prime_for_cuda_graph() or the step before the "
+                                       "capture had (or another graph holds them at other addresses): call prime_for_cuda_graph() "
+                                       "with the gradients in place, then capture")
                 if plan is not None:
-                    plan.close()
+                    self._drop(self.plans.pop(dev))
                 plan = DevicePlan(dev, es)
                 if self.push is not None:
                     plan.set_push(*self.push)
                 self.plans[dev] = plan
             ready.append(plan)
         for dev in [d for d in self.plans if d not in by_dev]:
-            self.plans.pop(dev).close()
+            self._drop(self.plans.pop(dev))
         return ready
 
     def set_hyper(self, hypers: list) -> None:
+        for plan in self.retired:      # (param_groups are only ever added)
+            plan.set_hyper(hypers[:plan.captured])
         for plan in self.plans.values():
             plan.set_hyper(hypers)
+
+    def last_captured(self) -> list:
+        """The plans of the latest capture."""
+        return [plan for plan in self.plans.values() if plan.captured] or self.retired[-1:]
 
     def step(self, entries: list, hypers: list) -> int:
         launches = 0

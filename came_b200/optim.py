@@ -383,7 +383,8 @@ class _CameB200Optimizer(torch.optim.Optimizer):
         weight_decay from `param_groups` and rewrites the records the captured step uploads at each replay, so a
         learning-rate schedule needs no re-capture.  (The reference's captured kernels carry these values as
         launch arguments and have to be captured again, CAME8bit2D.py:52-72.)  Call it before launching the
-        replay that should see the new values."""
+        replay that should see the new values.  The optimizer has to outlive its graphs: they read its plans, which it keeps
+        for them when gradients, parameters or states move to other addresses in later eager steps."""
         self._engine.set_hyper(self._hypers())
 
     # -- checkpointing --------------------------------------------------------------------------
@@ -394,6 +395,8 @@ class _CameB200Optimizer(torch.optim.Optimizer):
         """torch's loader casts every state tensor to the parameter's dtype, which destroys int8/uint8
         codes and fp32 absmax for bf16/fp16 parameters.  Reload, then restore each tensor with the dtype
         it was saved with, drop the reference's scratch keys and rebuild the flat-layout alias views."""
+        self._engine.invalidate()
+        self._table = None
         super().load_state_dict(state_dict)
         saved_groups = state_dict["param_groups"]
         saved_state = state_dict["state"]
@@ -412,8 +415,6 @@ class _CameB200Optimizer(torch.optim.Optimizer):
                     st[k] = copy.deepcopy(v)   # torch's loader turns str values such as "_mode" into garbage
             if st.get("_mode") == "full8bit" and st.get("factored", False) and "factored_row_q" in st:
                 bind_flat_views(st)
-        self._engine.invalidate()
-        self._table = None
 
     def add_param_group(self, param_group):
         super().add_param_group(param_group)

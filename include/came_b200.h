@@ -211,10 +211,13 @@ int came_b200_clip_grad_norm(const CameGradRef* grads, int n_tensors, float max_
  * came_b200_plan_set_hyper rewrites that copy (learning-rate schedules without re-capturing); it makes no CUDA
  * call that touches a stream.  The copy node reads the buffer when the graph runs, so rewrite it only when no
  * replay that should still see the old values is pending.  The gradient and parameter addresses are those of
- * the plan at capture time.  The reference bakes the learning rate into the captured kernel arguments
+ * the plan at capture time: from then on came_b200_plan_set_pointers refuses to move them.  A replay reads the plan's
+ * workspace and its page-locked records, so destroy the plan after the graph.  came_b200_plan_captured: the number of records
+ * that a captured step of the plan reads, 0 when none was captured.  The reference bakes the learning rate into the captured kernel arguments
  * (came_pytorch/CAME8bit2D.py:52-72 prime_for_cuda_graph, came_pytorch/CAME8bit.py:672-693).
  */
 int came_b200_plan_set_hyper(came_plan_t* plan, const CameHyper* hypers, int n_groups);
+int came_b200_plan_captured(const came_plan_t* plan);
 
 /*
  * Waits for `stream` and reads the plan's device status word: 0, or 1 when a kernel gave up waiting for a

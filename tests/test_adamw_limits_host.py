@@ -19,3 +19,55 @@ def test_clip_refuses_addresses_off_their_elements():
     for at, dtype in ((0x10001, _lib.DT_F32), (0x10002, _lib.DT_F32), (0x10001, _lib.DT_F16), (0x10003, _lib.DT_BF16)):
         assert code(at, dtype) == _lib.E_INVALID and b"aligned" in lib.came_b200_last_error()
     assert code(0x10000, _lib.DT_F32, norm=0x1002) == _lib.E_INVALID and b"aligned" in lib.came_b200_last_error()
+
+
+class _Plan:
+    """A plan as the engine sees it, without a device."""
+    made = []
+
+    def __init__(self, device, entries):
+        self.device, self.n, self.captured, self.open, self.records = device, len(entries), 0, True, None
+        self.structure = tuple(e.structure_key() for e in entries)
+        self.addresses = tuple((e.p.data_ptr(), e.g.data_ptr()) for e in entries)
+        _Plan.made.append(self)
+
+    def repoint(self, entries):
+        return self.addresses == tuple((e.p.data_ptr(), e.g.data_ptr()) for e in entries) or not self.captured
+
+    def set_hyper(self, records):
+        assert self.open
+        self.records = list(records)
+
+    def close(self):
+        self.open = False
+
+
+def test_a_captured_plan_is_never_closed(monkeypatch):
+    """A graph reads the workspace and the page-locked records of the plan it was captured from at every replay."""
+    from came_b200 import engine
+    monkeypatch.setattr(engine, "DevicePlan", _Plan)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    _Plan.made = []
+
+    def entries(flags=0):
+        t = [torch.zeros(4) for _ in range(4)]
+        return [engine.Entry(p=t[0], g=t[1], mode=_lib.MODE_ADAMW, flags=flags, group=0, m=t[2], sq_row=t[3], res_row=torch.zeros(()))]
+
+    e, first = engine.StepEngine(), entries()
+    e.prepare(first)
+    e.prepare(entries())                      # another set: the first plan goes
+    assert [p.open for p in _Plan.made] == [False, True]
+    _Plan.made[1].captured = 1
+    e.prepare(entries(_lib.F_ADAMW_CLIP))     # ... but not one that was captured
+    e.prepare(entries())
+    assert [p.open for p in _Plan.made] == [False, True, False, True]
+    _Plan.made[3].captured = 2
+    e.invalidate()
+    assert _Plan.made[3].open and not e.plans
+    e.prepare(first)
+    e.set_hyper(["a", "b", "c"])              # every graph sees a schedule
+    assert _Plan.made[1].records == ["a"] and _Plan.made[3].records == ["a", "b"] and _Plan.made[4].records == ["a", "b", "c"]
+    assert e.last_captured() == [_Plan.made[3]]
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="prime_for_cuda_graph"):
+        e.prepare(entries())
