@@ -196,6 +196,11 @@ class DevicePlan:
         _lib.check(self.lib.came_b200_plan_set_hyper(self.handle, arr, len(hypers)))
 
     @property
+    def clips(self) -> bool:
+        """Whether a step takes the norm of the gradients."""
+        return self.lib.came_b200_plan_norm_offset(self.handle) >= 0
+
+    @property
     def grad_norm(self):
         """The norm the last step clipped by, as a view of the workspace (None: the plan takes none)."""
         at = self.lib.came_b200_plan_norm_offset(self.handle)

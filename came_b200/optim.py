@@ -663,6 +663,7 @@ class AdamW(_CameB200Optimizer):
     max_grad_norm: clip by the norm N of all gradients of the optimizer (each times its group's grad_scale), as the step
     reads them: the gradients themselves are not written.  N is left in `grad_norm`.  With a norm that is not finite nothing
     is stepped and no count raised.  `math.inf` takes the norm without clipping.  All parameters have to be on one device.
+    In a captured step the limit may change (`update_captured_hypers()`), but not between a number and None.
 
     Parameters of any shape (empty ones are passed over).  States replaced by hand (not by load_state_dict) are seen after
     the next `prime_for_cuda_graph()`."""
@@ -711,11 +712,18 @@ class AdamW(_CameB200Optimizer):
         return self._layout, _lib.F_ADAMW_CLIP if self._max_grad_norm is not None else 0, 0
 
     def _hypers(self):
-        return [make_adamw_hyper(g["lr"], g["betas"], g["eps"], g["weight_decay"], self._max_grad_norm,
+        return [make_adamw_hyper(g["lr"], g["betas"], g["eps"], g["weight_decay"], *self._table_args(),
                                  float(g.get("grad_scale", 1.0))) for g in self.param_groups]
 
     def _table_args(self) -> tuple:
-        return (1.0 if self._max_grad_norm is None else self._max_grad_norm,)
+        return (math.inf if self._max_grad_norm is None else self._max_grad_norm,)
+
+    def update_captured_hypers(self) -> None:
+        for plan in self._engine.last_captured():
+            if plan.clips != (self._max_grad_norm is not None):
+                raise ValueError(f"the step was captured {'with' if plan.clips else 'without'} max_grad_norm, which is now {self._max_grad_norm}: "
+                                 "a captured step takes another limit, but whether it clips at all is part of the capture")
+        super().update_captured_hypers()
 
     _state_tensors = {"exp_avg": torch.float32, "exp_avg_sq": torch.float32}
 

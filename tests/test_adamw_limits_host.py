@@ -1,5 +1,6 @@
 """What the AdamW step and the gradient clip refuse, count and remember, on the CPU."""
 import ctypes as C
+import math
 
 import pytest
 import torch
@@ -71,3 +72,37 @@ def test_a_captured_plan_is_never_closed(monkeypatch):
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
     with pytest.raises(RuntimeError, match="prime_for_cuda_graph"):
         e.prepare(entries())
+
+
+@pytest.mark.parametrize("cls", [came_b200.AdamW, came_b200.AdamW8bit])
+def test_the_limit_of_a_captured_step(cls):
+    """Without a limit the record's is infinite (factor 1), and a captured step cannot be switched between the two."""
+    opt = cls([torch.nn.Parameter(torch.zeros(4))], max_grad_norm=5.0)
+    assert opt._hypers()[0].clip_threshold == 5.0
+    opt.max_grad_norm = None
+    assert opt._hypers()[0].clip_threshold == math.inf and opt._table_args() == (math.inf,)
+
+    class Plan:
+        def __init__(self, clips, captured):
+            self.clips, self.captured, self.records = clips, captured, None
+
+        def set_hyper(self, records):
+            self.records = records
+
+        def close(self):
+            pass
+
+    for clips in (False, True):
+        for retired in (False, True):      # (retired: an eager step has taken another plan since)
+            plan, other = Plan(clips, 1), Plan(not clips, 0)
+            opt._engine.retired = [plan] if retired else []
+            opt._engine.plans = {"cuda": other if retired else plan}
+            opt.max_grad_norm = 2.0 if clips else None
+            opt.update_captured_hypers()
+            assert plan.records[0].clip_threshold == (2.0 if clips else math.inf)
+            plan.records = None
+            opt.max_grad_norm = None if clips else 2.0
+            with pytest.raises(ValueError, match="captured"):
+                opt.update_captured_hypers()
+            assert plan.records is None
+    opt._engine.retired, opt._engine.plans = [], {}

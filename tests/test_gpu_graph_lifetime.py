@@ -144,3 +144,38 @@ def test_a_capture_that_would_need_a_new_plan_is_refused():
     second.replay()
     torch.cuda.synchronize()
     assert opt.state[ps[0]]["step"].item() == 2
+
+
+@pytest.mark.parametrize("name", ["AdamW", "AdamW8bit"])
+@pytest.mark.parametrize("limit", [None, 0.01])
+def test_the_clip_is_switched_around_a_capture(name, limit):
+    """The graph goes on as it was captured, eager steps follow the switch, and a schedule for the graph is refused."""
+    ps, qs = _params(), _params()
+    opt, twin = _make(name, ps, max_grad_norm=limit), _make(name, qs, max_grad_norm=limit)
+    gs = _grads(ps, 1)
+    for p, q, g in zip(ps, qs, gs):
+        p.grad = q.grad = g
+    opt.prime_for_cuda_graph()
+    graph = _capture(opt)
+    graph.replay()
+    twin.step()
+    for o in (opt, twin):
+        o.max_grad_norm = None if limit else 0.01
+    with pytest.raises(ValueError, match="captured"):
+        opt.update_captured_hypers()
+    opt.step(), twin.step()
+    with pytest.raises(ValueError, match="captured"):
+        opt.update_captured_hypers()
+    graph.replay()
+    twin.max_grad_norm = limit
+    twin.step()
+    torch.cuda.synchronize()
+    _same(ps, opt, qs, twin)
+    opt.prime_for_cuda_graph()
+    graph = _capture(opt)      # a capture of the new setting: it may be updated
+    opt.update_captured_hypers()
+    graph.replay()
+    twin.max_grad_norm = opt.max_grad_norm
+    twin.step()
+    torch.cuda.synchronize()
+    _same(ps, opt, qs, twin)
