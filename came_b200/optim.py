@@ -749,11 +749,12 @@ class AdamW(_CameB200Optimizer):
             raise RuntimeError(f"step has to be an fp32 tensor of one element on {p.device}")
 
     def _collect(self):
+        starts = [p.data_ptr() for g in self.param_groups for p in g["params"] if p.grad is not None and p.numel()]
+        if len(set(starts)) != len(starts):      # (the parameters themselves: a step may take copies of them)
+            raise ValueError("a parameter is listed twice: its two steps would race")
         entries, hypers, copy_backs = super()._collect()
         if self._max_grad_norm is not None and len({e.p.device for e in entries}) > 1:
             raise RuntimeError("max_grad_norm needs all parameters on one device")
-        if len({e.p.data_ptr() for e in entries}) != len(entries):
-            raise ValueError("a parameter is listed twice: its two steps would race")
         return entries, hypers, copy_backs
 
     def load_state_dict(self, state_dict):

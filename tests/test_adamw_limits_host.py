@@ -106,3 +106,24 @@ def test_the_limit_of_a_captured_step(cls):
                 opt.update_captured_hypers()
             assert plan.records is None
     opt._engine.retired, opt._engine.plans = [], {}
+
+
+@pytest.mark.filterwarnings("ignore:optimizer contains a parameter group with duplicate parameters")
+@pytest.mark.parametrize("cls", [came_b200.AdamW, came_b200.AdamW8bit])
+def test_a_parameter_listed_twice_is_refused_whatever_its_strides(cls):
+    """(a step takes a copy of a parameter that is not contiguous, but its states are one)"""
+    for p in (torch.nn.Parameter(torch.zeros(4, 6).t()), torch.nn.Parameter(torch.zeros(2, 3, 4, 4).to(memory_format=torch.channels_last)),
+              torch.nn.Parameter(torch.zeros(5))):
+        p.grad = torch.ones_like(p)
+        alias = torch.nn.Parameter(p.data)
+        alias.grad = p.grad
+        for twice in ([p, p], [p, alias]):
+            opt = cls(twice)
+            with pytest.raises(ValueError, match="twice"):
+                opt.step()
+            assert not opt.state      # refused before anything is made
+    empty = [torch.nn.Parameter(torch.zeros(0)) for _ in range(2)]
+    for p in empty:
+        p.grad = torch.zeros(0)
+    with pytest.raises(RuntimeError, match="CUDA"):      # (empty ones share no element)
+        cls(empty).step()
