@@ -275,7 +275,7 @@ size_t carve(const CameTensorDesc& d, const Geometry& g, const Context& ctx, flo
 int validate(const CameTensorDesc& d, int i) {
     if (!d.p || !d.g || !d.m) return fail(CAME_E_INVALID, "tensor %d: p, g and m must be non-null", i);
     if (d.rows <= 0 || d.cols < 0) return fail(CAME_E_INVALID, "tensor %d: bad shape [%lld, %lld]", i, (long long)d.rows, (long long)d.cols);
-    if (d.rows > 0x7fffffffLL || d.cols > 0x7fffffffLL) return fail(CAME_E_UNSUPPORTED, "tensor %d: dimension above 2^31-1", i);
+    if (!is_adamw(d) && (d.rows > 0x7fffffffLL || d.cols > 0x7fffffffLL)) return fail(CAME_E_UNSUPPORTED, "tensor %d: dimension above 2^31-1", i);
     if (d.mode < CAME_MODE_FP32 || d.mode > CAME_MODE_ADAMW8) return fail(CAME_E_INVALID, "tensor %d: bad mode %d", i, d.mode);
     if (d.p_dtype < CAME_DT_F32 || d.p_dtype > CAME_DT_BF16 || d.g_dtype < CAME_DT_F32 || d.g_dtype > CAME_DT_BF16)
         return fail(CAME_E_INVALID, "tensor %d: bad dtype", i);

@@ -137,11 +137,14 @@ class DevicePlan:
             d.sq_col, d.sq_col_absmax = _ptr(e.sq_col), _ptr(e.sq_col_absmax)
             d.res_row, d.res_row_absmax = _ptr(e.res_row), _ptr(e.res_row_absmax)
             d.res_col, d.res_col_absmax = _ptr(e.res_col), _ptr(e.res_col_absmax)
-            if e.p.dim() <= 1:
+            if elementwise or e.p.dim() == 1:      # (a count of 64 bits)
                 d.rows, d.cols, d.batch = e.p.numel(), 0, 0
             else:      # more than two dimensions: a batch of [shape[-2], shape[-1]] matrices
                 d.rows, d.cols = e.p.shape[-2], e.p.shape[-1]
-                d.batch = math.prod(e.p.shape[:-2]) if e.p.dim() > 2 else 0
+                batch = math.prod(e.p.shape[:-2]) if e.p.dim() > 2 else 0
+                if batch >= 1 << 32:      # (the field has 32 bits, and would keep the lower ones)
+                    raise RuntimeError(f"came_b200 steps at most 2^32 - 1 matrices of a parameter, got {batch}")
+                d.batch = batch
             d.mode, d.flags, d.group = e.mode, e.flags, e.group
             d.p_dtype, d.g_dtype = dtype_code(e.p.dtype), dtype_code(e.g.dtype)
         nbytes = self.lib.came_b200_workspace_bytes(descs, self.n)

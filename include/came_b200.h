@@ -39,7 +39,8 @@ enum {
                          /* with one absmax per 256 (came8bit2d_state.py:33-55)                                */
     CAME_MODE_FLAT8 = 2, /* CAME8bitFull / CAME8bitMemory, and every 1-D 8-bit tensor: int8 exp_avg with one   */
                          /* absmax per 256 flat elements, uint8 vectors (blockwise_quantization.py:17-27)      */
-    /* AdamW (no counterpart in the reference).  Element-wise: rows, cols and batch only give the element count. */
+    /* AdamW (no counterpart in the reference).  Element-wise: rows, cols and batch only give the element count, */
+    /* 4e12 at most; rows may hold all of it.                                                                        */
     CAME_MODE_ADAMW = 3, /* fp32 exp_avg (m) and exp_avg_sq (sq_row)                                           */
     CAME_MODE_ADAMW8 = 4 /* exp_avg: float8 e4m3 codes (m), exp_avg_sq: float8 e5m2 codes (sq_row), each with  */
                          /* one e8m0 byte (a power-of-two scale) per 256 flat elements in m_absmax / sq_row_absmax */

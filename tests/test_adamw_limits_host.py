@@ -127,3 +127,49 @@ def test_a_parameter_listed_twice_is_refused_whatever_its_strides(cls):
         p.grad = torch.zeros(0)
     with pytest.raises(RuntimeError, match="CUDA"):      # (empty ones share no element)
         cls(empty).step()
+
+
+def _table(monkeypatch, shape, mode):
+    """The row of the tensor table that DevicePlan makes of a parameter."""
+    from came_b200 import engine
+    rows = []
+
+    class Lib:
+        def came_b200_workspace_bytes(self, descs, n):
+            rows.extend((d.rows, d.cols, d.batch) for d in descs)
+            return 0
+
+    monkeypatch.setattr(engine._lib, "load", lambda: Lib())
+    monkeypatch.setattr(engine._lib, "check", lambda rc: (_ for _ in ()).throw(StopAsyncIteration))
+    t = [torch.empty(shape, device="meta") for _ in range(2)]
+    e = engine.Entry(p=t[0], g=t[1], mode=mode, flags=0, group=0, m=t[0], sq_row=t[0], res_row=t[0])
+    with pytest.raises(StopAsyncIteration):
+        engine.DevicePlan(torch.device("cpu"), [e])
+    return rows[0]
+
+
+def test_elements_are_counted_in_64_bits(monkeypatch):
+    lib = _lib.load()
+    size = lambda **kw: lib.came_b200_workspace_bytes((_lib.CameTensorDesc * 1)(_desc(**kw)), 1)  # noqa: E731
+    for mode in (_lib.MODE_ADAMW, _lib.MODE_ADAMW8):
+        assert size(mode=mode, rows=1 << 31, cols=0) > 0 and size(mode=mode, rows=(1 << 33) + 1, cols=0) > 0
+        assert size(mode=mode, rows=4_100_000_000_000, cols=0) == 0 and size(mode=mode, rows=1 << 62, cols=1 << 62) == 0
+        assert size(mode=mode, rows=1 << 62, cols=1, batch=(1 << 32) - 1) == 0
+    assert size(mode=_lib.MODE_FP32, rows=1 << 31, cols=0) == 0
+    with monkeypatch.context() as m:
+        for shape in ((1 << 32, 2, 2), (3, 1 << 31, 1, 1), ((1 << 31) + 5,), (5, 7), ()):
+            for mode in (_lib.MODE_ADAMW, _lib.MODE_ADAMW8):
+                assert _table(m, shape, mode) == (math.prod(shape), 0, 0)
+        assert _table(m, (3, 5, 7), _lib.MODE_FP32) == (5, 7, 3) and _table(m, (5, 7), _lib.MODE_FP32) == (5, 7, 0)
+        with pytest.raises(RuntimeError, match="matrices"):
+            _table(m, (1 << 32, 2, 2), _lib.MODE_FP32)
+
+
+def _desc(**kw):
+    d = _lib.CameTensorDesc()
+    for k, f in enumerate(("p", "g", "m", "m_absmax", "sq_row", "sq_row_absmax", "res_row")):
+        setattr(d, f, 0x10000 * (k + 1))
+    d.rows, d.cols, d.p_dtype, d.g_dtype = 64, 64, _lib.DT_BF16, _lib.DT_BF16
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
