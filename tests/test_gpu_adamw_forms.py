@@ -1,12 +1,34 @@
-"""AdamW and AdamW8bit where there are more than 2^31 elements."""
+"""AdamW and AdamW8bit where the element types of parameters and gradients differ, and where there are more than 2^31 elements."""
 import math
 
 import pytest
 import torch
 
-from tests.test_gpu_adamw import EPS24, _cls
+from tests.test_gpu_adamw import EPS24, HYPER, _check_step, _cls, _params
 
 pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+SHAPES = [(), (7,), (255,), (256,), (257,), (33, 770), (3, 5, 7), (130, 513), (64, 4096)]
+
+
+@pytest.mark.parametrize("limit", [None, 0.05])
+@pytest.mark.parametrize("p_packed,g_packed", [(False, False), (True, False), (False, True), (True, True)])
+@pytest.mark.parametrize("p_type,g_type", [(p, g) for p in TYPES for g in TYPES if p != g])
+@pytest.mark.parametrize("kind", ["fp32", "8bit"])
+def test_gradients_of_another_type(kind, p_type, g_type, p_packed, g_packed, limit):
+    """Every step against the definition, each side on vector boundaries or off them."""
+    ps = _params(SHAPES, p_type, packed=p_packed)
+    for p in ps:
+        p.grad_dtype = None      # (lifts the rule that both have one type)
+    opt = _cls(kind)(ps, **HYPER, max_grad_norm=limit)
+    for k in range(3):
+        gs = [g.data for g in _params(SHAPES, g_type, 20 + k, g_packed, 1e-2)]
+        for p, g in zip(ps, gs):
+            p.grad = g
+        norm = math.sqrt(sum((g.double() ** 2).sum().item() for g in gs))
+        c = 1.0 if limit is None else min(1.0, limit / (norm + 1e-6))
+        _check_step(opt, opt.step, c, 6 * EPS24 if c < 1.0 else 0.0)
 
 
 def _big(kind, shape, offset):
