@@ -44,7 +44,7 @@ struct Param {                    // (no reference to the parameter: swap_tensor
     at::ScalarType p_type, g_type;
     const void *p_ptr, *g_ptr;
     std::vector<int64_t> sizes;
-    int plan, pos;                // entry of a plan's tensor table
+    int plan, pos;                // entry of a plan's tensor table; none (-1): an empty parameter of AdamW
 };
 struct Plan {
     int device;
@@ -97,7 +97,8 @@ bool usable(const at::Tensor& p, const at::Tensor& g) {
 }
 
 // build(param_groups, [(DevicePlan, device index, n)], [state dict][, max_grad_norm of AdamW]): remembers the tensors of a step that the
-// Python path has just made.  Parameters with a gradient fill the plans' tables in order, by device.  False when they do not.
+// Python path has just made.  Parameters with a gradient (AdamW: and elements) fill the plans' tables in order, by device.  False when
+// they do not.
 bool build(StepTable* s, PyObject* groups, PyObject* plans, PyObject* states) {
     table_clear(s);
     std::vector<int> expect;
@@ -124,17 +125,20 @@ bool build(StepTable* s, PyObject* groups, PyObject* plans, PyObject* states) {
             if (g.defined()) {
                 int k = 0;
                 while (k < (int)s->plans->size() && (*s->plans)[k].device != t.device().index()) ++k;
-                if (k == (int)s->plans->size() || !usable(t, g)) { ok = false; break; }
-                Plan& plan = (*s->plans)[k];
+                const bool passed_over = s->adamw && t.numel() == 0;
+                if (!usable(t, g) || (k == (int)s->plans->size() && !passed_over)) { ok = false; break; }
                 e.has_grad = true;
                 e.p_type = t.scalar_type();
                 e.g_type = g.scalar_type();
                 e.p_ptr = t.const_data_ptr();
                 e.g_ptr = g.const_data_ptr();
                 e.sizes = t.sizes().vec();
-                e.plan = k;
-                e.pos = (int)plan.g.size();
-                plan.g.push_back(e.g_ptr);
+                if (!passed_over) {
+                    Plan& plan = (*s->plans)[k];
+                    e.plan = k;
+                    e.pos = (int)plan.g.size();
+                    plan.g.push_back(e.g_ptr);
+                }
             }
             ps.push_back(std::move(e));
         }
@@ -291,6 +295,7 @@ long step(StepTable* s, PyObject* groups) {
             if (!usable(t, g) || g.scalar_type() != e.g_type || t.scalar_type() != e.p_type || t.const_data_ptr() != e.p_ptr ||
                 t.sizes() != at::IntArrayRef(e.sizes) || g.device() != t.device())
                 return SLOW;
+            if (e.plan < 0) continue;
             const void* at = g.const_data_ptr();
             if (at != e.g_ptr) {
                 moved = true;

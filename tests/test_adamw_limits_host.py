@@ -173,3 +173,22 @@ def _desc(**kw):
     for k, v in kw.items():
         setattr(d, k, v)
     return d
+
+
+def test_an_empty_parameter_does_not_keep_the_table_away():
+    """AdamW passes over it: it has no place in the plan, and the table has to know."""
+    class Plan:
+        handle = None
+        addresses = ()
+
+    def build(sizes, n, *limit):
+        ps = [torch.nn.Parameter(torch.zeros(s)) for s in sizes]
+        for p in ps:
+            p.grad = torch.zeros_like(p)
+        groups = [dict(params=ps, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0)]
+        keep.append(ps)
+        return _host.StepTable().build(groups, [(Plan(), -1, n)], [], *limit)
+
+    keep = []
+    assert build([4], 1, 1.0) and build([4, 0], 1, 1.0) and build([0, 4, 0], 1, math.inf) and build([(3, 0, 2), 4, 5], 2, 1.0)
+    assert not build([4, 0], 2, 1.0) and not build([4, 5], 1, 1.0) and not build([4, 0], 1)      # (the last: a CAME table)

@@ -179,3 +179,20 @@ def test_the_clip_is_switched_around_a_capture(name, limit):
     twin.step()
     torch.cuda.synchronize()
     _same(ps, opt, qs, twin)
+
+
+@pytest.mark.parametrize("name", ["AdamW", "AdamW8bit"])
+def test_empty_parameters_step_by_the_table(name):
+    import came_b200
+    ps, qs = _params(), _params()
+    empty = [torch.nn.Parameter(torch.zeros(s, device="cuda", dtype=torch.bfloat16)) for s in ((0,), (4, 0))]
+    opt, twin = getattr(came_b200, name)([empty[0], *ps, empty[1]], lr=1e-3), getattr(came_b200, name)(qs, lr=1e-3)
+    for k in range(4):
+        for p, q, g in zip(ps, qs, _grads(ps, 5 + k)):
+            p.grad = q.grad = g
+        for e in empty:
+            e.grad = torch.zeros_like(e) if k != 2 else None
+        opt.step(), twin.step()
+        assert opt._table is not None
+    torch.cuda.synchronize()
+    _same(ps, opt, qs, twin)
