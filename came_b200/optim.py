@@ -704,9 +704,12 @@ class AdamW(_CameB200Optimizer):
     @property
     def grad_norm(self):
         """Norm of all gradients at the last step under `max_grad_norm`: a 0-dimensional fp32 tensor on the device, which the
-        next step overwrites (clone it to keep it).  None without `max_grad_norm`, and before the first step."""
+        next step overwrites (clone it to keep it).  None without `max_grad_norm`, and before the first step.  A captured step
+        writes the tensor that this gave right after the capture, also when eager steps with other tensors have one of their own."""
         plans = list(self._engine.plans.values())
-        return plans[0].grad_norm if self._max_grad_norm is not None and len(plans) == 1 else None
+        if self._max_grad_norm is None or len(plans) != 1 or plans[0].last_launches == 0:
+            return None
+        return plans[0].grad_norm
 
     def _route(self, p, grad, group):
         return self._layout, _lib.F_ADAMW_CLIP if self._max_grad_norm is not None else 0, 0

@@ -192,3 +192,19 @@ def test_an_empty_parameter_does_not_keep_the_table_away():
     keep = []
     assert build([4], 1, 1.0) and build([4, 0], 1, 1.0) and build([0, 4, 0], 1, math.inf) and build([(3, 0, 2), 4, 5], 2, 1.0)
     assert not build([4, 0], 2, 1.0) and not build([4, 5], 1, 1.0) and not build([4, 0], 1)      # (the last: a CAME table)
+
+
+def test_no_norm_before_the_first_step():
+    """(prime_for_cuda_graph() makes the plan, whose norm then is a zero that nobody took)"""
+    class Plan:
+        grad_norm, last_launches, captured = 0.0, 0, 0
+
+        def close(self):
+            pass
+
+    opt = came_b200.AdamW([torch.nn.Parameter(torch.zeros(4))], max_grad_norm=1.0)
+    opt._engine.plans = {"cuda": Plan()}
+    assert opt.grad_norm is None
+    opt._engine.plans["cuda"].last_launches = 2
+    assert opt.grad_norm == 0.0
+    opt._engine.plans = {}

@@ -196,3 +196,24 @@ def test_empty_parameters_step_by_the_table(name):
         assert opt._table is not None
     torch.cuda.synchronize()
     _same(ps, opt, qs, twin)
+
+
+@pytest.mark.parametrize("name", ["AdamW", "AdamW8bit"])
+def test_the_norm_belongs_to_its_plan(name):
+    ps = _params()
+    opt = _make(name, ps, max_grad_norm=1.0)
+    own = _grads(ps, 1)
+    for p, g in zip(ps, own):
+        p.grad = g
+    opt.prime_for_cuda_graph()
+    assert opt.grad_norm is None
+    graph = _capture(opt)
+    captured = opt.grad_norm
+    for p, g in zip(ps, _grads(ps, 2)):
+        p.grad = g * 3
+    opt.step()
+    graph.replay()
+    torch.cuda.synchronize()
+    for norm, gs in ((captured, own), (opt.grad_norm, [p.grad for p in ps])):
+        want = sum((g.double() ** 2).sum().item() for g in gs) ** 0.5
+        assert abs(norm.item() - want) <= 6 * 2.0 ** -24 * want
