@@ -12,6 +12,7 @@
 
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <c10/core/impl/COWDeleter.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -450,7 +451,10 @@ PyObject* clip_grad_norm(PyObject*, PyObject* args) {
     int of_params;
     if (!PyArg_ParseTuple(args, "O!dp", &PyList_Type, &list, &max_norm, &of_params)) return nullptr;
     std::vector<CameGradRef> refs;
+    std::vector<c10::TensorImpl*> scaled;      // written by an operation in place, as autograd has to know
+    const bool writes = !std::isinf(max_norm);
     at::Tensor first;
+    if (writes) scaled.reserve((size_t)PyList_GET_SIZE(list));
     refs.reserve((size_t)PyList_GET_SIZE(list));
     PyTypeObject* known = nullptr;      // asking whether a parameter is a tensor takes as long as the rest: once per type
     for (Py_ssize_t i = 0; i < PyList_GET_SIZE(list); ++i) {
@@ -462,15 +466,22 @@ PyObject* clip_grad_norm(PyObject*, PyObject* args) {
         const at::Tensor& t = THPVariable_Unpack(o);
         const at::Tensor& g = of_params ? t.grad() : t;
         if (!g.defined()) continue;
-        if (g.layout() != at::kStrided || !g.is_cuda() || (first.defined() && g.device() != first.device())) Py_RETURN_NONE;
+        c10::TensorImpl* const impl = g.unsafeGetTensorImpl();
+        // (a dense CUDA tensor)
+        if (!impl->key_set().has(c10::DispatchKey::CUDA) || (first.defined() && g.device() != first.device())) Py_RETURN_NONE;
         const at::ScalarType type = g.scalar_type();
         const int dtype = type == at::kFloat ? CAME_DT_F32 : type == at::kHalf ? CAME_DT_F16 : type == at::kBFloat16 ? CAME_DT_BF16 : -1;
         if (dtype < 0 || !g.is_non_overlapping_and_dense()) Py_RETURN_NONE;
         if (!first.defined()) first = g;
-        if (g.numel() > 0) refs.push_back(CameGradRef{const_cast<void*>(g.const_data_ptr()), g.numel(), dtype, 0});
+        if (g.numel() == 0) continue;
+        // (what a lazy copy shares is copied before it is written)
+        const bool shared = writes && impl->storage().data_ptr().get_deleter() == &c10::impl::cow::cow_deleter;
+        refs.push_back(CameGradRef{shared ? g.mutable_data_ptr() : const_cast<void*>(g.const_data_ptr()), g.numel(), dtype, 0});
+        if (writes && !impl->is_inference()) scaled.push_back(impl);
     }
     if (!first.defined()) Py_RETURN_NONE;
     if (listed_twice(refs)) Py_RETURN_NONE;
+    for (c10::TensorImpl* g : scaled) g->bump_version();
     at::Tensor norm;
     int rc;
     {
