@@ -2,6 +2,7 @@
 #pragma once
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "launch.h"
@@ -186,7 +187,9 @@ static cudaError_t launch_behind(void (*kernel)(P...), int grid, int threads, in
     c.stream = st;
     c.attrs = &early;
     c.numAttrs = 1;
-    return cudaLaunchKernelEx(&c, kernel, args...);
+    static_assert((std::is_same_v<P, A> && ...), "the arguments are passed by their addresses");
+    void* at[] = {const_cast<void*>(static_cast<const void*>(&args))...};      // (no copy of tables of 20 KB on the way)
+    return cudaLaunchKernelExC(&c, reinterpret_cast<const void*>(kernel), at);
 }
 // The beginning: the norm of all gradients.  False: it is not finite, and the step does not take place.
 __device__ __forceinline__ bool adamw_norm(const AdamwArgs& w, double* norm) {
