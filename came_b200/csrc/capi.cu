@@ -416,6 +416,7 @@ struct came_plan {
     // CUDA graph (the graph's copy node reads it again at every replay)
     CameHyper* graph_hyp = nullptr;
     int graph_groups = 0;
+    bool descs_pending = false;    // addresses set while a stream was captured: the next step uploads them
     int captured_groups = 0;       // records of a step that was captured: from then on the addresses stay
     ~came_plan() {
         for (auto& t : timed) { cudaEventDestroy(t.t0); cudaEventDestroy(t.t1); }
@@ -837,6 +838,21 @@ int came_b200_plan_pushed(const came_plan_t* plan, int* flags, int n_tensors) {
     return CAME_OK;
 }
 
+static bool is_capturing(cudaStream_t st) {
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(st, &cap) != cudaSuccess) { cudaGetLastError(); return false; }
+    return cap == cudaStreamCaptureStatusActive;
+}
+static cudaError_t upload_descs(const came_plan* plan, cudaStream_t st) {
+    // pageable copies up to 64 KB return as soon as they are staged; longer ones wait for the stream
+    const size_t total = (size_t)plan->n_tensors * sizeof(CameTensorDesc), piece = 48 * 1024;
+    const char* src = reinterpret_cast<const char*>(plan->descs.data());
+    cudaError_t e = cudaSuccess;
+    for (size_t at = 0; at < total && e == cudaSuccess; at += piece)
+        e = cudaMemcpyAsync(plan->ws + plan->L.off_descs + at, src + at, std::min(piece, total - at), cudaMemcpyHostToDevice, st);
+    return e;
+}
+
 int came_b200_plan_set_pointers(came_plan_t* plan, const void* const* g, void* const* p, int n_tensors, came_stream_t stream) {
     if (!plan) return fail(CAME_E_INVALID, "set_pointers: plan is null");
     if (n_tensors != plan->n_tensors) return fail(CAME_E_INVALID, "set_pointers: %d tensors given, plan has %d", n_tensors, plan->n_tensors);
@@ -862,15 +878,13 @@ int came_b200_plan_set_pointers(came_plan_t* plan, const void* const* g, void* c
         if (g) plan->descs[i].g = g[i];
         if (p) plan->descs[i].p = p[i];
     }
-    // pageable copies up to 64 KB return as soon as they are staged; longer ones wait for the stream
-    const size_t total = (size_t)n_tensors * sizeof(CameTensorDesc), piece = 48 * 1024;
-    const char* src = reinterpret_cast<const char*>(plan->descs.data());
-    for (size_t at = 0; at < total; at += piece) {
-        const cudaError_t e = cudaMemcpyAsync(plan->ws + plan->L.off_descs + at, src + at, std::min(piece, total - at),
-                                              cudaMemcpyHostToDevice, (cudaStream_t)stream);
-        if (e != cudaSuccess) return fail(CAME_E_CUDA, "set_pointers: %s", cudaGetErrorString(e));
+    if (is_capturing((cudaStream_t)stream)) {
+        plan->descs_pending = true;
+        return CAME_OK;
     }
-    return CAME_OK;
+    plan->descs_pending = false;
+    const cudaError_t e = upload_descs(plan, (cudaStream_t)stream);
+    return e == cudaSuccess ? CAME_OK : fail(CAME_E_CUDA, "set_pointers: %s", cudaGetErrorString(e));
 }
 
 int came_b200_plan_set_hyper(came_plan_t* plan, const CameHyper* hypers, int n_groups) {
@@ -889,9 +903,7 @@ int came_b200_step(came_plan_t* plan, const CameHyper* hypers, int n_groups, cam
     cudaStream_t st = (cudaStream_t)stream;
     // While the stream is being captured into a CUDA graph the upload must read memory that outlives the call:
     // the plan's page-locked copy, which came_b200_plan_set_hyper rewrites between replays.
-    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-    if (cudaStreamIsCapturing(st, &cap) != cudaSuccess) { cap = cudaStreamCaptureStatusNone; cudaGetLastError(); }
-    const bool capturing = cap == cudaStreamCaptureStatusActive;
+    const bool capturing = is_capturing(st);
     CameHyper norm[MAX_GROUPS];      // pageable source: read before the copy call returns
     std::memcpy(norm, hypers, (size_t)n_groups * sizeof(CameHyper));
     normalise_hypers(norm, n_groups);
@@ -907,6 +919,11 @@ int came_b200_step(came_plan_t* plan, const CameHyper* hypers, int n_groups, cam
     const bool by_value = !capturing && n_groups <= GENERIC_MAX_HYP;
     static_assert(GENERIC_MAX_HYP == ADAMW_MAX_HYP, "one rule for the records that travel as arguments");
     cudaError_t e = cudaSuccess;
+    if (plan->descs_pending) {      // (a captured upload has run only when its graph has)
+        e = upload_descs(plan, st);
+        if (e != cudaSuccess) return fail(CAME_E_CUDA, "step: upload of the addresses: %s", cudaGetErrorString(e));
+        plan->descs_pending = capturing;
+    }
     if (plan->needs_hyp || !by_value) {
         e = cudaMemcpyAsync(plan->ws + plan->L.off_hyp, src, (size_t)n_groups * sizeof(CameHyper), cudaMemcpyHostToDevice, st);
         if (e != cudaSuccess) return fail(CAME_E_CUDA, "step: hyper-parameter upload: %s", cudaGetErrorString(e));

@@ -159,7 +159,8 @@ int came_b200_plan_create(const CameTensorDesc* descs, int n_tensors, void* work
 void came_b200_plan_destroy(came_plan_t* plan);
 
 /* Re-point the gradients (and parameters, when non-NULL) of an existing plan: the analogue of
- * fill_device_ptr_tensor (came_bindings.cpp:461-478).  Arrays of n_tensors device pointers, host memory. */
+ * fill_device_ptr_tensor (came_bindings.cpp:461-478).  Arrays of n_tensors device pointers, host memory.  While `stream` is
+ * being captured nothing is enqueued: the steps that follow, captured or not, upload the addresses. */
 int came_b200_plan_set_pointers(came_plan_t* plan, const void* const* g, void* const* p, int n_tensors,
                                 came_stream_t stream);
 

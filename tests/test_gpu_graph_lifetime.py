@@ -217,3 +217,42 @@ def test_the_norm_belongs_to_its_plan(name):
     for norm, gs in ((captured, own), (opt.grad_norm, [p.grad for p in ps])):
         want = sum((g.double() ** 2).sum().item() for g in gs) ** 0.5
         assert abs(norm.item() - want) <= 6 * 2.0 ** -24 * want
+
+
+@pytest.mark.parametrize("name", ["AdamW8bit", "CAME8bit"])
+def test_an_eager_step_between_a_capture_with_other_gradients_and_its_first_replay(name):
+    """The capture moves the plan to other gradients, but its upload of their addresses has not run yet."""
+    ps, qs = _params(), _params()
+    opt, twin = _make(name, ps), _make(name, qs)
+    first, gs = _grads(ps, 1), _grads(ps, 2)
+    for p, g in zip(ps, first):
+        p.grad = g
+    opt.prime_for_cuda_graph()
+    for p, q, g in zip(ps, qs, gs):
+        p.grad = q.grad = g
+    graphs = [_capture(opt), _capture(opt)]      # (the second finds the plan moved)
+    opt.step(), twin.step()
+    torch.cuda.synchronize()
+    _same(ps, opt, qs, twin)
+    for graph in graphs:
+        graph.replay()
+        twin.step()
+    torch.cuda.synchronize()
+    _same(ps, opt, qs, twin)
+
+
+@pytest.mark.parametrize("name", ["AdamW8bit", "CAME8bit"])
+def test_two_captures_with_other_gradients_before_any_step(name):
+    ps, qs = _params(), _params()
+    opt, twin = _make(name, ps), _make(name, qs)
+    first, gs = _grads(ps, 1), _grads(ps, 2)
+    for p, g in zip(ps, first):
+        p.grad = g
+    opt.prime_for_cuda_graph()
+    for p, q, g in zip(ps, qs, gs):
+        p.grad = q.grad = g
+    _, second = _capture(opt), _capture(opt)
+    second.replay()      # the first never runs
+    twin.step()
+    torch.cuda.synchronize()
+    _same(ps, opt, qs, twin)
