@@ -261,11 +261,20 @@ came_plan_t* handle_of(const Plan& plan) {
     return static_cast<came_plan_t*>(p);
 }
 
+size_t records_of(const StepTable* s, size_t n_groups) { return (s->adamw ? 1 : 2) * n_groups; }
+bool fill_records(StepTable* s, PyObject* groups, CameHyper* out) {
+    for (Py_ssize_t gi = 0; gi < PyList_GET_SIZE(groups); ++gi) {
+        PyObject* const group = PyList_GET_ITEM(groups, gi);
+        if (!(s->adamw ? adamw_hyper_of(s, group, out + gi) : hypers_of(s, group, out + 2 * gi))) return false;
+    }
+    return true;
+}
+
 // step(param_groups): launches (>= 0), SLOW or FAILED + code
 long step(StepTable* s, PyObject* groups) {
     if (s->plans->empty() || !PyList_Check(groups) || (size_t)PyList_GET_SIZE(groups) != s->groups->size()) return SLOW;
     const size_t n_groups = s->groups->size();
-    const size_t records = (s->adamw ? 1 : 2) * n_groups;
+    const size_t records = records_of(s, n_groups);
     if (records > 64) return SLOW;
     // (what is used without the lock below: the table may be dropped or rebuilt by another thread meanwhile)
     struct Target {
@@ -311,12 +320,10 @@ long step(StepTable* s, PyObject* groups) {
         if (!v || !(PyLong_CheckExact(v) || PyFloat_CheckExact(v))) return SLOW;
     }
     CameHyper hyp[64];
-    for (size_t gi = 0; gi < n_groups; ++gi)
-        if (!(s->adamw ? adamw_hyper_of(s, PyList_GET_ITEM(groups, (Py_ssize_t)gi), hyp + gi)
-                       : hypers_of(s, PyList_GET_ITEM(groups, (Py_ssize_t)gi), hyp + 2 * gi))) {
-            PyErr_Clear();      // the Python path raises what there is to raise
-            return SLOW;
-        }
+    if (!fill_records(s, groups, hyp)) {
+        PyErr_Clear();      // the Python path raises what there is to raise
+        return SLOW;
+    }
     if (moved) {
         for (size_t k = 0; k < targets.size(); ++k) {
             if (PyObject_SetAttrString(targets[k].plan.get(), "addresses", Py_None) != 0) return SLOW;
@@ -354,6 +361,20 @@ PyObject* table_step(PyObject* self, PyObject* groups) {
     return PyLong_FromLong(r);
     END_HANDLE_TH_ERRORS
 }
+// records(param_groups): the hyper-parameter records that step() would pass, as bytes; None where it would hand over
+PyObject* table_records(PyObject* self, PyObject* groups) {
+    HANDLE_TH_ERRORS
+    StepTable* s = reinterpret_cast<StepTable*>(self);
+    CameHyper hyp[64];
+    if (!PyList_Check(groups) || records_of(s, (size_t)PyList_GET_SIZE(groups)) > 64) Py_RETURN_NONE;
+    if (!fill_records(s, groups, hyp)) {
+        PyErr_Clear();
+        Py_RETURN_NONE;
+    }
+    return PyBytes_FromStringAndSize(reinterpret_cast<const char*>(hyp),
+                                     (Py_ssize_t)(records_of(s, (size_t)PyList_GET_SIZE(groups)) * sizeof(CameHyper)));
+    END_HANDLE_TH_ERRORS
+}
 PyObject* table_forget(PyObject* self, PyObject*) {
     table_clear(reinterpret_cast<StepTable*>(self));
     Py_RETURN_NONE;
@@ -361,6 +382,7 @@ PyObject* table_forget(PyObject* self, PyObject*) {
 
 PyMethodDef table_methods[] = {{"build", table_build, METH_VARARGS, "remember the tensors of a step"},
                                {"step", table_step, METH_O, "step them again; launches, -1 (slow path) or -1000 + code"},
+                               {"records", table_records, METH_O, "the records of a step as bytes, or None"},
                                {"forget", table_forget, METH_NOARGS, "drop every reference"},
                                {nullptr, nullptr, 0, nullptr}};
 PyTypeObject table_type = {PyVarObject_HEAD_INIT(nullptr, 0)};

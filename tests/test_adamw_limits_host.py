@@ -208,3 +208,39 @@ def test_no_norm_before_the_first_step():
     opt._engine.plans["cuda"].last_launches = 2
     assert opt.grad_norm == 0.0
     opt._engine.plans = {}
+
+
+@pytest.mark.parametrize("limit", [None, 1.0, 0.37, math.inf])
+def test_records_of_the_native_table_equal_those_of_the_python_path(limit):
+    """Byte for byte, AdamW's one per group and CAME's two."""
+    from came_b200.engine import make_adamw_hyper, make_hyper
+    p = torch.nn.Parameter(torch.zeros(4))
+    p.grad = torch.zeros(4)
+
+    class Plan:
+        handle = None
+        addresses = ()
+
+    def records(groups, *args):
+        table = _host.StepTable()
+        assert table.build(groups, [(Plan(), -1, 1)], [], *args)
+        return table.records(groups)
+
+    ps = [[p], [], []]
+    groups = [dict(params=ps[0], lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.1),
+              dict(params=ps[1], lr=3e-4, betas=[0.0, 0.95], eps=1e-30, weight_decay=0.0, grad_scale=1.0 / 1024),
+              dict(params=ps[2], lr=0, betas=(0.95, 0.0), eps=0.0, weight_decay=1, grad_scale=3)]
+    bound = math.inf if limit is None else limit
+    want = b"".join(bytes(make_adamw_hyper(g["lr"], g["betas"], g["eps"], g["weight_decay"], bound, float(g.get("grad_scale", 1.0))))
+                    for g in groups)
+    assert records(groups, bound) == want
+    opt = came_b200.AdamW([dict(g, params=[torch.nn.Parameter(torch.zeros(1))]) for g in groups], max_grad_norm=limit)
+    assert b"".join(bytes(h) for h in opt._hypers()) == want
+    table = _host.StepTable()
+    assert table.build(groups, [(Plan(), -1, 1)], [], bound)
+    assert table.records(groups * 22) is None      # (66 of 64)
+    groups[1]["betas"] = (0.9, 1.0)
+    assert table.records(groups) is None      # (the Python path raises)
+    came = [dict(params=ps[0], lr=1e-3, betas=(0.9, 0.999, 0.9999), eps=(1e-30, 1e-16), clip_threshold=1.0, weight_decay=0.1, grad_scale=0.5)]
+    want = b"".join(bytes(make_hyper(1e-3, (0.9, 0.999, 0.9999), (1e-30, 1e-16), 1.0, 0.1, python_scalars=k, grad_scale=0.5)) for k in (False, True))
+    assert records(came) == want
