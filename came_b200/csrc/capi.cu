@@ -4,8 +4,9 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <exception>
 #include <map>
-#include <new>
+#include <memory>
 #include <tuple>
 #include <vector>
 
@@ -486,8 +487,8 @@ size_t came_b200_workspace_bytes(const CameTensorDesc* descs, int n_tensors) {
     return layout(descs, n_tensors, context(descs, n_tensors)).total;
 }
 
-int came_b200_plan_create(const CameTensorDesc* descs, int n_tensors, void* workspace, size_t workspace_bytes,
-                          came_stream_t stream, came_plan_t** out) {
+static int plan_create(const CameTensorDesc* descs, int n_tensors, void* workspace, size_t workspace_bytes,
+                       came_stream_t stream, came_plan_t** out) {
     if (!out) return fail(CAME_E_INVALID, "plan_create: out is null");
     *out = nullptr;
     if (!descs || n_tensors <= 0) return fail(CAME_E_INVALID, "plan_create: no tensors");
@@ -509,8 +510,7 @@ int came_b200_plan_create(const CameTensorDesc* descs, int n_tensors, void* work
     if (workspace_bytes < L.total)
         return fail(CAME_E_WORKSPACE, "plan_create: workspace of %zu bytes, %zu needed", workspace_bytes, L.total);
 
-    came_plan* plan = new (std::nothrow) came_plan();
-    if (!plan) return fail(CAME_E_INVALID, "plan_create: out of host memory");
+    auto plan = std::make_unique<came_plan>();
     plan->n_tensors = n_tensors;
     plan->descs.assign(descs, descs + n_tensors);
     plan->ws = static_cast<char*>(workspace);
@@ -765,10 +765,7 @@ int came_b200_plan_create(const CameTensorDesc* descs, int n_tensors, void* work
         build(KID_APPLY_FLAT, in_flat, [&](int i) { return Key{D[i].g_dtype, D[i].p_dtype, 0, 2}; }, tiles);
     }
 
-    if (work.size() > L.n_work) {
-        delete plan;
-        return fail(CAME_E_INVALID, "plan_create: internal work-list overflow (%zu > %zu)", work.size(), L.n_work);
-    }
+    if (work.size() > L.n_work) return fail(CAME_E_INVALID, "plan_create: internal work-list overflow (%zu > %zu)", work.size(), L.n_work);
 
     cudaStream_t st = (cudaStream_t)stream;
     cudaError_t e = cudaMemcpyAsync(plan->ws + L.off_descs, plan->descs.data(), (size_t)n_tensors * sizeof(CameTensorDesc),
@@ -784,14 +781,19 @@ int came_b200_plan_create(const CameTensorDesc* descs, int n_tensors, void* work
     if (e == cudaSuccess) e = cudaStreamSynchronize(st);
     if (e == cudaSuccess)
         e = cudaHostAlloc(reinterpret_cast<void**>(&plan->graph_hyp), (size_t)MAX_GROUPS * sizeof(CameHyper), cudaHostAllocDefault);
-    if (e != cudaSuccess) {
-        delete plan;
-        return fail(CAME_E_CUDA, "plan_create: %s", cudaGetErrorString(e));
-    }
+    if (e != cudaSuccess) return fail(CAME_E_CUDA, "plan_create: %s", cudaGetErrorString(e));
     for (const LaunchItem& it : plan->launches)
         plan->needs_hyp = plan->needs_hyp || (it.kernel != KID_GENERIC && it.kernel != KID_ADAMW && it.kernel != KID_ADAMW8 && it.kernel != KID_GRAD_NORM);
-    *out = plan;
+    *out = plan.release();
     return CAME_OK;
+}
+int came_b200_plan_create(const CameTensorDesc* descs, int n_tensors, void* workspace, size_t workspace_bytes,
+                          came_stream_t stream, came_plan_t** out) {
+    try {      // (no exception leaves a C entry)
+        return plan_create(descs, n_tensors, workspace, workspace_bytes, stream, out);
+    } catch (const std::exception& e) {
+        return fail(CAME_E_INVALID, "plan_create: out of host memory (%s)", e.what());
+    }
 }
 
 void came_b200_plan_destroy(came_plan_t* plan) { delete plan; }

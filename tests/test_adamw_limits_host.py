@@ -1,6 +1,8 @@
 """What the AdamW step and the gradient clip refuse, count and remember, on the CPU."""
 import ctypes as C
 import math
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -244,3 +246,26 @@ def test_records_of_the_native_table_equal_those_of_the_python_path(limit):
     came = [dict(params=ps[0], lr=1e-3, betas=(0.9, 0.999, 0.9999), eps=(1e-30, 1e-16), clip_threshold=1.0, weight_decay=0.1, grad_scale=0.5)]
     want = b"".join(bytes(make_hyper(1e-3, (0.9, 0.999, 0.9999), (1e-30, 1e-16), 1.0, 0.1, python_scalars=k, grad_scale=0.5)) for k in (False, True))
     assert records(came) == want
+
+
+def test_a_plan_beyond_the_hosts_memory_is_an_error():
+    """4e12 elements are two billion work items: the list of them does not fit what the process may have, and no exception (which
+    would end the process) leaves the C entry."""
+    code = """
+import ctypes as C, importlib.util, resource, sys
+spec = importlib.util.spec_from_file_location("_lib", sys.argv[1])
+_lib = importlib.util.module_from_spec(spec)
+spec.loader.exec_module(_lib)
+lib = _lib.load()
+used = int(open("/proc/self/statm").read().split()[0]) * resource.getpagesize()
+resource.setrlimit(resource.RLIMIT_AS, (used + (2 << 30),) * 2)
+d = _lib.CameTensorDesc()
+for k, f in enumerate(("p", "g", "m", "m_absmax", "sq_row", "sq_row_absmax", "res_row")):
+    setattr(d, f, 0x10000 * (k + 1))
+d.rows, d.cols, d.mode, d.p_dtype, d.g_dtype = 4000000000000, 0, _lib.MODE_ADAMW8, _lib.DT_BF16, _lib.DT_BF16
+plan = C.c_void_p()
+rc = lib.came_b200_plan_create((_lib.CameTensorDesc * 1)(d), 1, 0x10000000, 1 << 60, None, C.byref(plan))
+print(rc, plan.value, lib.came_b200_last_error().decode())
+"""
+    out = subprocess.run([sys.executable, "-c", code, _lib.__file__], capture_output=True, text=True, timeout=120)
+    assert out.returncode == 0 and out.stdout.startswith(f"{_lib.E_INVALID} None") and "memory" in out.stdout, (out.returncode, out.stdout, out.stderr)
