@@ -268,8 +268,10 @@ class StepEngine:
     def _drop(self, plan) -> None:
         if plan.captured:
             self.retired.append(plan)
-        else:
-            plan.close()
+            return
+        if plan.last_launches:      # its steps may still run, on any stream, and read a workspace that the next allocation gets
+            torch.cuda.synchronize(plan.device)
+        plan.close()
 
     def invalidate(self) -> None:
         while self.plans:

@@ -29,7 +29,7 @@ class _Plan:
     made = []
 
     def __init__(self, device, entries):
-        self.device, self.n, self.captured, self.open, self.records = device, len(entries), 0, True, None
+        self.device, self.n, self.captured, self.open, self.records, self.last_launches = device, len(entries), 0, True, None, 0
         self.structure = tuple(e.structure_key() for e in entries)
         self.addresses = tuple((e.p.data_ptr(), e.g.data_ptr()) for e in entries)
         _Plan.made.append(self)
@@ -74,6 +74,21 @@ def test_a_captured_plan_is_never_closed(monkeypatch):
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
     with pytest.raises(RuntimeError, match="prime_for_cuda_graph"):
         e.prepare(entries())
+
+
+def test_a_plan_whose_steps_may_still_run_is_waited_for(monkeypatch):
+    """It may have been stepped on another stream than the one its workspace was allocated on."""
+    from came_b200 import engine
+    done = []
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda device=None: done.append(device))
+    monkeypatch.setattr(_Plan, "close", lambda self: done.append("closed"))
+    e = engine.StepEngine()
+    for launches in (0, 2):
+        plan = _Plan("cuda:3", [])
+        plan.last_launches = launches
+        e.plans["cuda:3"] = plan
+        e.invalidate()
+    assert done == ["closed", "cuda:3", "closed"]
 
 
 @pytest.mark.parametrize("cls", [came_b200.AdamW, came_b200.AdamW8bit])
