@@ -387,6 +387,20 @@ class _CameB200Optimizer(torch.optim.Optimizer):
         for them when gradients, parameters or states move to other addresses in later eager steps."""
         self._engine.set_hyper(self._hypers())
 
+    # -- copies and pickles ---------------------------------------------------------------------
+    def __getstate__(self):
+        """What torch keeps, and the settings of the classes; not the plans, which a copy makes anew."""
+        settings = {k: v for k, v in self.__dict__.items() if k not in ("_table", "last_step_launches") and
+                    (v is None or isinstance(v, (bool, int, float, str, tuple)))}
+        return {**settings, **super().__getstate__()}
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        if "_engine" not in self.__dict__:      # (torch's load_state_dict comes here as well)
+            self._engine = StepEngine()
+            self.last_step_launches = 0
+        self._table = None
+
     # -- checkpointing --------------------------------------------------------------------------
     def state_dict(self):
         return super().state_dict()

@@ -181,7 +181,7 @@ int came_b200_step(came_plan_t* plan, const CameHyper* hypers, int n_groups, cam
  * least normal number that of the subnormals, 2^-9 resp. 2^-16): 0 <= r < 1 is r = (s mod 2^20) / 2^20 (m), (s >> 11) / 2^21
  * (v), with s = mix((e >> 3) + mix(t)) * (0x9E3779B1 * (2 (e & 7) + 1)) mod 2^32, e the flat index of the element and mix the
  * 32-bit mixer x ^= x >> 16, x *= 0x7feb352d, x ^= x >> 15, x *= 0x846ca68b, x ^= x >> 16.  A moment that is NaN is held as some
- * value, one that is infinite as the block's largest code or next to it.
+ * value; one that is infinite makes the scale its block's largest, so that the block's other moments fall to the least codes.
  * The norm N of the last step lies in the workspace, at the byte offset that came_b200_plan_norm_offset gives (one fp32
  * number; -1 when the plan takes none).
  */

@@ -1,6 +1,8 @@
 """What the AdamW step and the gradient clip refuse, count and remember, on the CPU."""
+import copy
 import ctypes as C
 import math
+import pickle
 import subprocess
 import sys
 
@@ -284,3 +286,19 @@ print(rc, plan.value, lib.came_b200_last_error().decode())
 """
     out = subprocess.run([sys.executable, "-c", code, _lib.__file__], capture_output=True, text=True, timeout=120)
     assert out.returncode == 0 and out.stdout.startswith(f"{_lib.E_INVALID} None") and "memory" in out.stdout, (out.returncode, out.stdout, out.stderr)
+
+
+@pytest.mark.parametrize("name,kw", [("AdamW", dict(max_grad_norm=0.5)), ("AdamW8bit", {}), ("CAME8bit", dict(cuda_1d_runtime_mode="repeated_fp16_pairmin"))])
+def test_copies_and_pickles_keep_the_settings(name, kw):
+    p = torch.nn.Parameter(torch.zeros(4, 4))
+    opt = getattr(came_b200, name)([p], lr=1e-3, **kw)
+    for other in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        assert other._engine is not opt._engine and other.param_groups[0]["lr"] == 1e-3 and other.last_step_launches == 0
+        for key in ("_max_grad_norm", "cuda_nonfactored_use_fp16_update", "prefer_cuda_2d_fast_path"):
+            assert getattr(other, key, "none") == getattr(opt, key, "none")
+        other.param_groups[0]["params"][0].grad = torch.ones(4, 4)
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            other.step()
+    engine = opt._engine
+    opt.load_state_dict(opt.state_dict())
+    assert opt._engine is engine      # (with the plans that graphs read)

@@ -256,3 +256,20 @@ def test_two_captures_with_other_gradients_before_any_step(name):
     twin.step()
     torch.cuda.synchronize()
     _same(ps, opt, qs, twin)
+
+
+@pytest.mark.parametrize("name", ["AdamW8bit", "CAME8bitFull"])
+def test_a_copy_goes_on_like_the_original(name):
+    opt = _make(name, _params())
+    ps = opt.param_groups[0]["params"]
+    for p, g in zip(ps, _grads(ps, 1)):
+        p.grad = g
+    opt.step()
+    other = copy.deepcopy(opt)
+    qs = other.param_groups[0]["params"]
+    for p, q, g in zip(ps, qs, _grads(ps, 2)):
+        p.grad = q.grad = g
+    opt.step(), other.step()
+    torch.cuda.synchronize()
+    assert all(p is not q for p, q in zip(ps, qs))
+    _same(ps, opt, qs, other)
