@@ -302,10 +302,8 @@ class StepEngine:
         return ready
 
     def set_hyper(self, hypers: list) -> None:
-        for plan in self.retired:      # (param_groups are only ever added)
-            plan.set_hyper(hypers[:plan.captured])
-        for plan in self.plans.values():
-            plan.set_hyper(hypers)
+        for plan in (*self.retired, *self.plans.values()):
+            plan.set_hyper(hypers[:plan.captured or None])      # (param_groups are only ever added)
 
     def last_captured(self) -> list:
         """The plans of the latest capture."""

@@ -72,6 +72,10 @@ def test_a_captured_plan_is_never_closed(monkeypatch):
     e.prepare(first)
     e.set_hyper(["a", "b", "c"])              # every graph sees a schedule
     assert _Plan.made[1].records == ["a"] and _Plan.made[3].records == ["a", "b"] and _Plan.made[4].records == ["a", "b", "c"]
+    _Plan.made[4].captured = 2                # (a group was added since)
+    e.set_hyper(["d", "e", "f"])
+    assert _Plan.made[4].records == ["d", "e"]
+    _Plan.made[4].captured = 0
     assert e.last_captured() == [_Plan.made[3]]
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
     with pytest.raises(RuntimeError, match="prime_for_cuda_graph"):
