@@ -14,8 +14,8 @@
 //
 // Bound by instructions first, by DRAM close behind (10.03 bytes an element in 16-bit types): one element per lane and step takes
 // 54 instructions; packed arithmetic, whole blocks without questions per block (span8_fast) and codes that are cut out of the
-// rounded bits instead of converted leave 33.  256 M bf16 elements: 405 us (97 % of the copy rate); under the power cap, back to
-// back, the clock falls to 1.6-1.8 GHz and 1.26 G elements take 2.06-2.2 ms (88-94 %).
+// rounded bits instead of converted leave 34.  256 M bf16 elements: 404 us (97 % of the copy rate); under the power cap, back to
+// back, the clock falls to 1.6-1.8 GHz and 1.26 G elements take 2.14-2.19 ms (88-90 %).
 #include <cfloat>
 
 #include "adamw.cuh"
@@ -24,8 +24,8 @@
 
 namespace came {
 
-// Two CTAs of 8 warps per SM and a ring of four slots: more warps mean fewer registers (80 at three CTAs: spills, 470 us where two
-// take 424 for 256 M bf16 elements), deeper rings bring nothing (five slots: 409 us, four: 406).
+// Two CTAs of 8 warps per SM and a ring of four slots: more warps mean fewer registers (80 at three CTAs: spills, 461 us where two
+// take 404 for 256 M bf16 elements), deeper rings bring nothing (five slots: 416 us).
 constexpr int ADAMW8_CTAS = 2, ADAMW8_STAGES = 4;
 // The fast root takes what is below 1.2e-38 for zero, the true one 1.1e-19 at most: with eps 2^24 times that (times the factor of
 // the root) or more, no digit of their sum is lost.
@@ -376,8 +376,8 @@ template <typename P, typename G> struct LaunchAdamw8 {
         constexpr int smem = Ring8<P, G>::CTA_BYTES;
         const cudaError_t e = cudaFuncSetAttribute(k_adamw8<P, G>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e != cudaSuccess) return e;
-        // Spans (256 M elements): 16-bit types are bound by instructions, a long span fills its ring less often (406 us with 16
-        // items, 429 with 8, 511 with 4); fp32 is bound by DRAM, which likes addresses close together (682, 658, 641).
+        // Spans (256 M elements): 16-bit types are bound by instructions, a long span fills its ring less often (404 us with 16
+        // items, 426 with 8, 509 with 4); fp32 is bound by DRAM, which likes addresses close together (683, 661, 642).
         AdamwArgs x = w;
         const int grid = adamw_spans(x, ADAMW8_CTAS, sizeof(P) + sizeof(G) <= 4 ? 16 : 4);
         return launch_behind(k_adamw8<P, G>, grid, ADAMW_THREADS, smem, st, a, x, h);
