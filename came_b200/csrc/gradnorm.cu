@@ -204,7 +204,7 @@ cudaError_t launch_clip(const CameGradRef* grads, int n, float max_norm, float* 
     double total = 0.0;
     for (int i = 0; i < n; ++i) total += (double)grads[i].n;
     int64_t chunk = 4096;
-    while (chunk < 65536 && total / (double)chunk > 2.0 * 148) chunk *= 2;
+    while (chunk < 65536 && total / (double)chunk > 2.0 * persistent_grid_limit()) chunk *= 2;
     while (total / (double)chunk > (double)(1 << 30)) chunk *= 2;
     int n_parts = 0;
     cudaError_t e = cudaSuccess;
